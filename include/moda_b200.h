@@ -208,6 +208,88 @@ int moda_b200_depth_take(const moda_problem *prob, const moda_tensor4 *grad_k,
                          const moda_tensor4 *grad_v, int32_t layer, const moda_tensor4 *d_k,
                          const moda_tensor4 *d_v, void *stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Serving: rotary positions, a paged KV cache, and the attention of one new token.  The reference has no
+ * counterpart (its operators take whole sequences); names and layouts follow the operators above.
+ * Of moda_problem these calls use B, T_kv, H, D, G, dtype and device, and L and scale where said.
+ * ------------------------------------------------------------------------------------------------ */
+
+/* How vectors turn with their position: pair i at position p by the angle p * inv_freq[i]. */
+typedef struct moda_rotary {
+  const double *inv_freq; /* DEVICE: rotary_dim / 2 frequencies, radians a position                      */
+  int32_t rotary_dim;     /* elements of a head that turn, its first ones: a multiple of 16, at most D    */
+  int32_t interleaved;    /* 0: pairs (i, i + rotary_dim / 2); otherwise pairs (2 i, 2 i + 1)             */
+  float scale;            /* factor on the turned elements (1; more where long contexts ask for it)      */
+} moda_rotary;
+
+/* Positions of tokens [B, T]: of a DEVICE tensor of whole numbers, or (data NULL) t + offset. */
+typedef struct moda_positions {
+  const void *data;
+  int64_t stride_b, stride_t; /* in elements, any (0: the same for all)  */
+  int64_t offset;
+  int32_t is_int64;           /* 0: int32                                */
+} moda_positions;
+
+/* Sequences whose K/V live in pages of a pool.  Row n of sequence b is row n % page_size of page
+ * block_table[b * table_stride + n / page_size]. */
+typedef struct moda_paged_cache {
+  moda_tensor4 k, v;          /* [num_pages, page_size, H, D]: stride_b of a page, stride_t of a row      */
+  int32_t num_pages, page_size;
+  const int32_t *block_table; /* DEVICE [B, max_pages]                                                   */
+  int64_t table_stride;
+  int32_t max_pages;
+  const int32_t *seq_lens;    /* DEVICE [B]: rows that the sequences hold before the call                 */
+} moda_paged_cache;
+
+/* Depth rows of the new tokens.  [B, L, H, D], the rows of a token's own position (positions_per_sequence = 1);
+ * or, chunk-visible, of P positions each (position p of a sequence lies p * stride_position further), of which
+ * sequence b sees the first positions_seen[b]. */
+typedef struct moda_depth_rows {
+  moda_tensor4 k, v;
+  int64_t k_stride_position, v_stride_position;
+  int32_t positions_per_sequence;
+  const int32_t *positions_seen; /* DEVICE [B]; NULL: all                                                 */
+} moda_depth_rows;
+
+/*
+ * Rotary positions of q [B, T_kv*G, H, D] (row t*G + g stands at position t) and, unless k is NULL, of
+ * k [B, T_kv, H, D], into q_out and k_out.  inverse != 0 turns the other way: the gradient's map.
+ * positions NULL: token t stands at position t.  An output may be its own input (same strides).
+ */
+int moda_b200_rotary(const moda_problem *prob, const moda_rotary *rot, const moda_positions *positions,
+                     int inverse, const moda_tensor4 *q, const moda_tensor4 *k,
+                     const moda_tensor4 *q_out, const moda_tensor4 *k_out, void *stream);
+
+/*
+ * Writes k, v [B, T_kv, H, D] into the cache behind what the sequences hold: token t of sequence b becomes row
+ * seq_lens[b] + t, for t < lengths[b] (DEVICE [B]; NULL: all T_kv).  Keys are turned on the way when rot
+ * is not NULL, at the position that is their row.  seq_lens stays as it is.  Rows that are to be written must
+ * lie in pages of one sequence only.  A token whose page is none of the pool's, or whose row the table does not
+ * cover, is left out and recorded (moda_b200_device_status).
+ */
+int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, const moda_tensor4 *v,
+                           const moda_paged_cache *cache, const int32_t *lengths, const moda_rotary *rot,
+                           void *stream);
+
+/*
+ * Attention of one new token (prob->T_kv = 1): q [B, G, H, D] sees, under one softmax, the seq_lens[b] cached
+ * rows of its sequence, its own k, v [B, 1, H, D] unless k is NULL, and the depth rows (prob->L layers; L = 0:
+ * none).  o [B, G, H, D], lse fp32 [B, G, H] in base-2 units; a token that sees nothing gets o = 0, lse = -inf.
+ * With k, v the call also appends them, as moda_b200_paged_append does, and unless k_copy is NULL writes the rows
+ * (the key turned) to k_copy, v_copy [B, 1, H, D] as well: a layer's slot of a depth cache.  With rot, q and k are
+ * turned: at position seq_lens[b] with k, v, and otherwise at seq_lens[b] - 1, that of the sequence's last row.
+ * Rows in pages that are none of the pool's are left out and recorded, as are lengths that are negative or
+ * more than the table covers.
+ * The results do not depend on scheduling.  workspace: caller-owned DEVICE scratch, 256-byte aligned,
+ * contents undefined on entry and exit; calls that may overlap on the GPU need one each.
+ */
+int moda_b200_paged_decode_workspace_bytes(const moda_problem *prob, size_t *bytes);
+int moda_b200_paged_decode(const moda_problem *prob, const moda_tensor4 *q, const moda_paged_cache *cache,
+                           const moda_tensor4 *k, const moda_tensor4 *v, const moda_tensor4 *k_copy,
+                           const moda_tensor4 *v_copy, const moda_depth_rows *depth, const moda_rotary *rot,
+                           const moda_tensor4 *o, float *lse, void *workspace, size_t workspace_bytes,
+                           void *stream);
+
 /*
  * Validation only (no launch): the status moda_b200_fwd / moda_b200_bwd would return
  * for this problem's shape fields.  Mirrors the reference's shape assertions
@@ -240,8 +322,10 @@ const char *moda_b200_kernel_name(int kernel_id);
  * unwritten.  The word is sticky: launches never clear it, it keeps the FIRST failure
  * since it was last read, and this call returns it and resets it to 0.  A caller that
  * wants to know that its results are valid reads it at its next synchronisation point
- * (0 = every launch since the previous read ran to completion).  SYNCHRONISES the
- * device.  The reference has no counterpart (Triton kernels do not spin on barriers
+ * (0 = every launch since the previous read ran to completion).  The paged-cache calls
+ * record here what they left out: (2 << 8 | 1) a page that is none of the pool's, (2 << 8 | 2) a
+ * length that is negative or more than the table covers; where both kinds were recorded the next call
+ * returns the second.  SYNCHRONISES the device.  The reference has no counterpart (Triton kernels do not spin on barriers
  * they could miss).
  */
 int moda_b200_device_status(int *status);

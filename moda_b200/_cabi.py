@@ -29,6 +29,10 @@ EXPORTED_SYMBOLS = (
     "moda_b200_bwd_static_scratch",
     "moda_b200_depth_append",
     "moda_b200_depth_take",
+    "moda_b200_rotary",
+    "moda_b200_paged_append",
+    "moda_b200_paged_decode_workspace_bytes",
+    "moda_b200_paged_decode",
     "moda_b200_check_problem",
     "moda_b200_resolve_path",
     "moda_b200_profile_begin",
@@ -71,6 +75,27 @@ class Problem(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):        # moda_rotary
+    _fields_ = [("inv_freq", ctypes.c_void_p), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("scale", ctypes.c_float)]
+
+
+class Positions(ctypes.Structure):         # moda_positions
+    _fields_ = [("data", ctypes.c_void_p), ("stride_b", ctypes.c_int64), ("stride_t", ctypes.c_int64),
+                ("offset", ctypes.c_int64), ("is_int64", ctypes.c_int32)]
+
+
+class PagedCache(ctypes.Structure):        # moda_paged_cache
+    _fields_ = [("k", Tensor4), ("v", Tensor4), ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
+                ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int32),
+                ("seq_lens", ctypes.c_void_p)]
+
+
+class DepthRows(ctypes.Structure):         # moda_depth_rows
+    _fields_ = [("k", Tensor4), ("v", Tensor4), ("k_stride_position", ctypes.c_int64), ("v_stride_position", ctypes.c_int64),
+                ("positions_per_sequence", ctypes.c_int32), ("positions_seen", ctypes.c_void_p)]
+
+
 class ModaLibraryError(RuntimeError):
     """The shared library is missing or returned a non-zero status."""
 
@@ -105,6 +130,15 @@ def load() -> ctypes.CDLL:
     lib.moda_b200_depth_append.restype = ctypes.c_int
     lib.moda_b200_depth_take.argtypes = [P, T, T, ctypes.c_int32, T, T, V]
     lib.moda_b200_depth_take.restype = ctypes.c_int
+    R, C, W = ctypes.POINTER(RotaryArgs), ctypes.POINTER(PagedCache), ctypes.POINTER(DepthRows)
+    lib.moda_b200_rotary.argtypes = [P, R, ctypes.POINTER(Positions), ctypes.c_int, T, T, T, T, V]
+    lib.moda_b200_rotary.restype = ctypes.c_int
+    lib.moda_b200_paged_append.argtypes = [P, T, T, C, V, R, V]
+    lib.moda_b200_paged_append.restype = ctypes.c_int
+    lib.moda_b200_paged_decode_workspace_bytes.argtypes = [P, ctypes.POINTER(ctypes.c_size_t)]
+    lib.moda_b200_paged_decode_workspace_bytes.restype = ctypes.c_int
+    lib.moda_b200_paged_decode.argtypes = [P, T, C, T, T, T, T, W, R, T, V, V, ctypes.c_size_t, V]
+    lib.moda_b200_paged_decode.restype = ctypes.c_int
     lib.moda_b200_check_problem.argtypes = [P]
     lib.moda_b200_check_problem.restype = ctypes.c_int
     lib.moda_b200_resolve_path.argtypes = [P, ctypes.c_int]
@@ -166,10 +200,10 @@ def profile_end() -> dict:
     """{kernel name: (launches, total_ms)} for the kernels launched since profile_begin."""
     lib = load()
     n = ctypes.c_int(0)
-    ids = (ctypes.c_int * 16)()
-    cnt = (ctypes.c_int * 16)()
-    ms = (ctypes.c_float * 16)()
-    check(lib.moda_b200_profile_end(16, ctypes.byref(n), ids, cnt, ms), "moda_b200_profile_end")
+    ids = (ctypes.c_int * 32)()
+    cnt = (ctypes.c_int * 32)()
+    ms = (ctypes.c_float * 32)()
+    check(lib.moda_b200_profile_end(32, ctypes.byref(n), ids, cnt, ms), "moda_b200_profile_end")
     return {lib.moda_b200_kernel_name(ids[i]).decode(): (int(cnt[i]), float(ms[i])) for i in range(n.value)}
 
 
@@ -184,11 +218,12 @@ def tensor_pipe_rates(device_ptr: int, device: int, stream: int = 0) -> None:
 
 
 def device_status() -> int:
-    """Sticky status word of the tcgen05 kernels' bounded waits; synchronises.
+    """Sticky status word of the tcgen05 kernels' bounded waits and of the paged-cache calls; synchronises.
 
     0 = every launch since the previous read ran to completion.  Non-zero = the first wait that
     expired since then ((1 << 8) | barrier id): that launch returned early and left outputs
-    unwritten.  Reading resets the word, so callers poll it at their next synchronisation point."""
+    unwritten; or what a paged-cache call left out first ((2 << 8) | 1: a page that is none of the
+    pool's, (2 << 8) | 2: a length that is negative or more than the table covers).  Reading resets the word, so callers poll it at their next synchronisation point."""
     v = ctypes.c_int(0)
     check(load().moda_b200_device_status(ctypes.byref(v)), "moda_b200_device_status")
     return int(v.value)

@@ -1,0 +1,509 @@
+// Attention of one new token over its sequence in a paged KV cache and the depth rows of earlier layers.
+//
+// For a sequence b and KV head h the G query heads see one list of keys: the sequence's rows (through the
+// block table), then the depth rows.  With s_j = scale q . k_j:  o = sum_j 2^(s_j log2 e - m) v_j / l, lse = m + log2 l,
+// in one pass with the running maximum m and sum l.  Every key row is read once for all G queries: 4 D G
+// flops for 4 D bytes, so the call is bound by memory up to G = 64 or so, and what the kernel is built for is to
+// have bytes on the way at all times:
+//
+//  - The work, 16-key tiles of every (b, h) in one row, is divided evenly between the CTAs by the lengths on
+//    the device (nothing is known on the host, and a captured call must follow new lengths).  A CTA walks its
+//    range, which may end one unit, hold several and begin another.  A unit that lies in one CTA's range is
+//    written at once, the others' parts are joined by a second, dependent launch.
+//  - A warp takes every fourth tile of the CTA's range.  Its lanes copy exactly the chunks that they
+//    will multiply, asynchronously, into slots of shared memory of their own, kStages tiles ahead and across the ends of
+//    units: no lane waits for another, so there are no barriers in the loop and no bank conflicts.
+//  - The products are m16n8k16 matrix instructions.  At 16 keys a tile and 8 query rows their rate is far from a
+//    limit (32 instructions a tile of 8 KB at D = 128), so that tcgen05 tiles of 128 keys, which need barriers, TMEM and
+//    16 times the padding, would buy nothing.  The order of the head's elements within a product and the order of V's
+//    columns are free, and are chosen so that each operand is a 16-byte chunk of a row: K: lane (g, t) = (lane / 4,
+//    lane % 4) holds elements 32 j + 8 t .. + 7 of key g; V: elements 64 j + 8 g .. + 7 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+//  - Eight query rows leave the lower half of the 16-row operand free.  It holds what rounding the upper half to 16
+//    bits has left over: the rotated query's remainder (the query is turned here, in 32 bits, without rounding), and that of
+//    the probabilities.  So neither is rounded to fewer than 16 significant bits, at no cost.
+#pragma once
+#include "rotary_kernels.cuh"
+
+namespace moda {
+namespace paged {
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kTile = 16;          // keys of a warp's step
+constexpr int kQ = 8;              // query heads of a unit; more are further units
+constexpr int kMinTiles = 8;       // a CTA's range is not made shorter: two tiles a warp
+
+struct DecodeParams {
+  View q, o;                       // [B, G, H, D]
+  Pages pages;
+  View kd, vd;                     // depth rows (b, layer, h); position p of P lies p * depth_sp further
+  int64_t kd_sp, vd_sp;
+  const int* depth_positions;      // [B]: positions seen, nullptr: all P
+  int P, L;
+  FastDiv by_L;
+  float* lse;                      // [B, G, H]
+  rotary::Args rot;                // of the queries, at the last position of the sequence
+  int B, H, G;
+  int own_key;                     // 1: the sequences hold one row more than seq_lens says (written by this call)
+  float scale_log2;
+  // scratch
+  int2* parts;                     // [CTA]: unit that is begun there and goes on in the next ones, and in how many it lies (0: none)
+  float2* ml;                      // [CTA][2][kQ]: maximum and sum; part 0 goes on from the CTA before, part 1 begins here
+  float* acc;                      // [CTA][2][kQ][D]
+};
+
+template <typename T> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two values as 16 bits each, and what that leaves over.
+template <typename T> __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = Pack<T>::pack(a, b);
+  const float2 r = Pack<T>::unpack(hi);
+  lo = Pack<T>::pack(a - r.x, b - r.y);
+}
+// 16 bytes from global memory to shared memory; !valid: zeros, and nothing is read.
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool valid) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t at) {
+  uint4 x;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+  return x;
+}
+
+template <int D> __host__ __device__ constexpr int stage_bytes() { return kTile * D * 2 * 2; }
+template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }      // 24 KB a warp
+// The copies' slots and the warps' parts of a unit.  With what the kernel declares statically, two CTAs just fit an SM.
+template <int D> constexpr size_t smem_bytes() { return (size_t)kWarps * stages<D>() * stage_bytes<D>() + (size_t)kWarps * kQ * D * 4; }
+// Four elements from 4 chunk on of a row of those parts; the order of a row's chunks spreads the lanes over the banks.
+template <int D> __device__ __forceinline__ float4* part_at(float* parts, int warp, int row, int chunk) {
+  return reinterpret_cast<float4*>(parts + (warp * kQ + row) * D) + (chunk ^ row);
+}
+
+struct Sequence { int len, keys, tiles; };          // rows in the cache, with the depth rows, 16-key tiles (at least one)
+__device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
+  Sequence s;
+  const int len = p.pages.seq_lens[b], room = p.pages.capacity();
+  s.len = len < 0 ? 0 : len >= room ? room : len + p.own_key;
+  const int P = p.depth_positions != nullptr ? min(max(p.depth_positions[b], 0), p.P) : p.P;
+  const int64_t keys = (int64_t)s.len + (int64_t)P * p.L;
+  s.keys = (int)(keys < 0x7ffffff0 ? keys : 0x7ffffff0);
+  s.tiles = max((s.keys + kTile - 1) / kTile, 1);
+  return s;
+}
+
+// A CTA's walk over its range of tiles: (sequence, unit of it, tiles [t0, t1) of the unit).
+struct Walk {
+  int b, unit;                       // unit: head * query blocks + query block
+  Sequence s;
+  int t0, t1;
+  int64_t left;                      // tiles of the range from t0 on
+  __device__ __forceinline__ void cut() { t1 = (int)min((int64_t)s.tiles, t0 + left); }
+  __device__ __forceinline__ bool next(const DecodeParams& p, int units) {
+    left -= t1 - t0;
+    if (left <= 0) return false;
+    if (++unit == units) { unit = 0; ++b; s = sequence(p, b); }
+    t0 = 0;
+    cut();
+    return true;
+  }
+};
+
+// The tiles of all units in a row, and this CTA's range of them.
+struct Range { int64_t total, begin, end; int n_cta; };
+template <int W> __device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* s_part) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (threadIdx.x % 32 == 0) s_part[threadIdx.x / 32] = x;
+  __syncthreads();
+  int64_t sum = 0;
+#pragma unroll
+  for (int i = 0; i < W; ++i) sum += s_part[i];
+  __syncthreads();
+  return sum;
+}
+__device__ __forceinline__ Walk locate(const DecodeParams& p, int units, Range& r) {
+  __shared__ int64_t s_part[kWarps];
+  __shared__ int s_b;
+  __shared__ int64_t s_first;
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0)
+    for (int b = tid; b < p.B; b += kThreads) {
+      const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : 0;
+      if (len < 0 || len > p.pages.capacity() - p.own_key || seen < 0 || seen > p.P) wrong(kBadLength);
+    }
+  const int tiles0 = tid < p.B ? sequence(p, tid).tiles : 0;
+  int64_t sum = tiles0;
+  for (int b = tid + kThreads; b < p.B; b += kThreads) sum += sequence(p, b).tiles;
+  r.total = block_sum<kWarps>(sum, s_part) * units;
+  r.n_cta = (int)min((int64_t)gridDim.x, (r.total + kMinTiles - 1) / kMinTiles);
+  const int i = blockIdx.x;
+  r.begin = r.end = 0;
+  Walk w{};
+  if (i >= r.n_cta) return w;
+  // total i / n without overflow: total below 2^47
+  r.begin = r.total / r.n_cta * i + r.total % r.n_cta * i / r.n_cta;
+  r.end = r.total / r.n_cta * (i + 1) + r.total % r.n_cta * (i + 1) / r.n_cta;
+  int64_t before = 0;
+  for (int base = 0;; base += kThreads) {                       // the sequence that holds tile `begin`
+    const int b = base + tid;
+    const int tiles = base == 0 ? tiles0 : b < p.B ? sequence(p, b).tiles : 0;
+    int64_t incl = (int64_t)tiles * units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (tid % 32 >= o) incl += up;
+    }
+    if (tid % 32 == 31) s_part[tid / 32] = incl;
+    __syncthreads();
+    int64_t start = before;
+    for (int j = 0; j < tid / 32; ++j) start += s_part[j];
+    const int64_t first = start + incl - (int64_t)tiles * units;
+    if (r.begin >= first && r.begin < start + incl) { s_b = b; s_first = first; }
+#pragma unroll
+    for (int j = 0; j < kWarps; ++j) before += s_part[j];
+    __syncthreads();
+    if (r.begin < before || base + kThreads >= p.B) break;      // uniform
+  }
+  w.b = s_b;
+  w.s = sequence(p, w.b);
+  const int64_t off = r.begin - s_first;
+  w.unit = (int)(off / w.s.tiles);
+  w.t0 = (int)(off % w.s.tiles);
+  w.left = r.end - r.begin;
+  w.cut();
+  return w;
+}
+
+// Copies the tiles of one warp, ahead of their use.
+template <int D> struct Loader {
+  Walk w;
+  int tile;                          // this warp's next one, of w
+  int page;                          // of this lane's key in it, fetched ahead
+  bool more;
+  uint32_t slot0;                    // this lane's first 16 bytes of stage 0
+  int stage;
+
+  __device__ __forceinline__ void settle(const DecodeParams& p, int units, int warp) {      // at a tile of this warp, or at the end
+    while (more && tile >= w.t1) {
+      more = w.next(p, units);
+      tile = w.t0 + warp;
+    }
+    fetch_page(p);
+  }
+  __device__ __forceinline__ void fetch_page(const DecodeParams& p) {
+    const int key = tile * kTile + (threadIdx.x & 15);
+    page = 0;
+    if (more && key < w.s.len) page = __ldg(p.pages.table + w.b * p.pages.table_stride + p.pages.by_page.div((uint32_t)key));
+  }
+  __device__ __forceinline__ void start(const DecodeParams& p, int units, int warp, const Walk& from, uint32_t ring) {
+    w = from; more = w.left > 0; tile = w.t0 + warp; stage = 0;
+    slot0 = ring + (threadIdx.x & 31) * 16;
+    settle(p, units, warp);
+  }
+  // Issues the copies of one tile (none at the end); `mask` in shared memory gets a bit for each key that is there.
+  __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, int warp, uint32_t* masks) {
+    if (more) {
+      const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+      const int key = tile * kTile + (lane & 15), h = w.unit / query_blocks;
+      const bool of_v = lane >= 16;
+      const View &cache = of_v ? p.pages.v : p.pages.k, &depth = of_v ? p.vd : p.kd;
+      bool valid = key < w.s.keys;
+      const unsigned char* row = static_cast<const unsigned char*>(cache.ptr);
+      if (key < w.s.len) {
+        if (page >= 0 && page < p.pages.num_pages) {
+          const int slot = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
+          row += 2 * cache.off(page, slot, h);
+        } else {
+          valid = false;
+          wrong(kBadPage);
+        }
+      } else if (valid) {
+        const int c = key - w.s.len, pos = (int)p.by_L.div((uint32_t)c), layer = c - pos * p.L;
+        row = static_cast<const unsigned char*>(depth.ptr) + 2 * (depth.off(w.b, layer, h) + pos * (of_v ? p.vd_sp : p.kd_sp));
+      }
+      const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu;
+      if (lane == 0) masks[stage] = there;
+      const uint32_t slot = slot0 + stage * stage_bytes<D>();
+      const unsigned long long at = reinterpret_cast<unsigned long long>(row);
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const unsigned long long k = __shfl_sync(0xffffffffu, at, nt * 8 + g) + t * 16;
+        const bool ok = (there >> (nt * 8 + g)) & 1u;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) copy16(slot + (nt * (D / 32) + j) * 512, reinterpret_cast<const void*>(k + j * 64), ok);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int vk = 2 * t + (i & 1) + (i >> 1) * 8;
+        const unsigned long long v = __shfl_sync(0xffffffffu, at, 16 + vk) + g * 16;
+        const bool ok = (there >> vk) & 1u;
+#pragma unroll
+        for (int j = 0; j < D / 64; ++j) copy16(slot + kTile * D * 2 + (i * (D / 64) + j) * 512, reinterpret_cast<const void*>(v + j * 128), ok);
+      }
+      tile += kWarps;
+      settle(p, units, warp);
+    }
+    copies_commit();
+    stage = stage + 1 == stages<D>() ? 0 : stage + 1;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ DecodeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint32_t s_masks[kWarps][stages<D>()];
+  __shared__ float2 s_ml[kWarps][kQ];
+  __shared__ float2 s_cs[D / 2];
+  constexpr int kStages = stages<D>();
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
+  const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
+  float* s_acc = reinterpret_cast<float*>(smem + (size_t)kWarps * kStages * stage_bytes<D>());
+
+  grid_started();
+  Range range;
+  Walk w = locate(p, units, range);
+  if (range.begin == range.end) {
+    if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
+    return;
+  }
+  Loader<D> loader;
+  loader.start(p, units, warp, w, ring);
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) loader.issue(p, units, query_blocks, warp, s_masks[warp]);
+
+  int stage = 0, turned_b = -1;
+  int64_t at = range.begin;                  // the walk's place in the row of all tiles
+  int2 part = make_int2(0, 0);
+  bool going = true;
+  while (going) {
+    const int h = w.unit / query_blocks, q0 = (w.unit - h * query_blocks) * kQ;
+    const bool row_there = q0 + g < p.G;
+    if (p.rot.inv_freq != nullptr && turned_b != w.b) {
+      __syncthreads();
+      for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], (long long)w.s.len - 1);
+      __syncthreads();
+      turned_b = w.b;
+    }
+    // this lane's part of the queries, in two 16-bit halves
+    uint32_t qh[D / 32][4], ql[D / 32][4];
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      const int chunk = 4 * j + t;
+      uint4 x = make_uint4(0, 0, 0, 0);
+      const int64_t row = p.q.off(w.b, q0 + g, h);
+      if (row_there) x = *rotary::chunk_at(p.q, row, chunk);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { qh[j][e] = (&x.x)[e]; ql[j][e] = 0; }
+      if (p.rot.inv_freq != nullptr && row_there && chunk * 8 < p.rot.rot) {
+        float y[8];
+        if (p.rot.interleaved) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = Pack<T>::unpack(qh[j][e]), cs = s_cs[chunk * 4 + e];
+            y[2 * e] = fmaf(a.x, cs.x, -a.y * cs.y);
+            y[2 * e + 1] = fmaf(a.y, cs.x, a.x * cs.y);
+          }
+        } else {
+          const int half = p.rot.rot >> 4;                     // chunks
+          const bool second = chunk >= half;
+          const uint4 other = *rotary::chunk_at(p.q, row, second ? chunk - half : chunk + half);
+          const int pair = (second ? chunk - half : chunk) * 8;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = Pack<T>::unpack(qh[j][e]), b = Pack<T>::unpack((&other.x)[e]);
+            const float2 c0 = s_cs[pair + 2 * e], c1 = s_cs[pair + 2 * e + 1];
+            y[2 * e] = fmaf(a.x, c0.x, second ? b.x * c0.y : -b.x * c0.y);
+            y[2 * e + 1] = fmaf(a.y, c1.x, second ? b.y * c1.y : -b.y * c1.y);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) split<T>(y[2 * e], y[2 * e + 1], qh[j][e], ql[j][e]);
+      }
+    }
+
+    float m = -INFINITY, l = 0.f;
+    float acc[D / 8][4];
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+
+    for (int tile = w.t0 + warp; tile < w.t1; tile += kWarps) {
+      copies_wait<kStages - 1>();
+      __syncwarp();                          // the mask is lane 0's
+      const uint32_t mask = s_masks[warp][stage];
+      const uint32_t slot = ring + stage * stage_bytes<D>() + lane * 16;
+      float s[2][4];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint4 k = lds128(slot + (nt * (D / 32) + j) * 512);
+          mma<T>(s[nt], qh[j][0], ql[j][0], qh[j][1], ql[j][1], k.x, k.y);
+          mma<T>(s[nt], qh[j][2], ql[j][2], qh[j][3], ql[j][3], k.z, k.w);
+        }
+      }
+      float x[4];                            // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool there = (mask >> (2 * t + (i & 1) + (i >> 1) * 8)) & 1u;
+        x[i] = there ? (s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)]) * p.scale_log2 : -INFINITY;
+      }
+      float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(top, m);
+      const float base = top == -INFINITY ? 0.f : top;
+      if (__any_sync(0xffffffffu, top > m)) {
+        const float shrink = fast_exp2(m - base);
+        l *= shrink;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) { acc[n][0] *= shrink; acc[n][1] *= shrink; acc[n][2] *= shrink; acc[n][3] *= shrink; }
+        m = top;
+      }
+      float pr[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { pr[i] = fast_exp2(x[i] - base); l += pr[i]; }
+      uint32_t ph[2], pl[2];
+      split<T>(pr[0], pr[1], ph[0], pl[0]);
+      split<T>(pr[2], pr[3], ph[1], pl[1]);
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = lds128(slot + kTile * D * 2 + (i * (D / 64) + j) * 512);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t a = (&v[0].x)[e], b = (&v[1].x)[e], c = (&v[2].x)[e], d = (&v[3].x)[e];
+          mma<T>(acc[j * 8 + 2 * e], ph[0], pl[0], ph[1], pl[1], __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
+          mma<T>(acc[j * 8 + 2 * e + 1], ph[0], pl[0], ph[1], pl[1], __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
+        }
+      }
+      __syncwarp();
+      loader.issue(p, units, query_blocks, warp, s_masks[warp]);
+      stage = stage + 1 == kStages ? 0 : stage + 1;
+    }
+
+    // the warps' parts
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    __syncthreads();                         // the part before has been read
+    if (t == 0) s_ml[warp][g] = make_float2(m, l);
+    if (row_there) {
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {        // column 2 t of product e is element 64 j + 16 t + e, column 2 t + 1 is 8 further
+          auto of = [&](int e) { return acc[j * 8 + (i & 1) * 4 + e][i >> 1] + acc[j * 8 + (i & 1) * 4 + e][2 + (i >> 1)]; };
+          *part_at<D>(s_acc, warp, g, 16 * j + 4 * t + i) = make_float4(of(0), of(1), of(2), of(3));
+        }
+    }
+    __syncthreads();
+    const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
+    constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
+    const int r = tid / 16, d0 = (tid % 16) * kEach;
+    if (q0 + r < p.G) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i][r].x);
+      const float base = top == -INFINITY ? 0.f : top;
+      float sum = 0.f, out[kEach] = {};
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const float weight = fast_exp2(s_ml[i][r].x - base);
+        sum = fmaf(s_ml[i][r].y, weight, sum);
+#pragma unroll
+        for (int e = 0; e < kEach; e += 4) {
+          const float4 x = *part_at<D>(s_acc, i, r, (d0 + e) / 4);
+          out[e] = fmaf(x.x, weight, out[e]);
+          out[e + 1] = fmaf(x.y, weight, out[e + 1]);
+          out[e + 2] = fmaf(x.z, weight, out[e + 2]);
+          out[e + 3] = fmaf(x.w, weight, out[e + 3]);
+        }
+      }
+      if (from_start && to_end) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint32_t packed[kEach / 2];
+#pragma unroll
+        for (int e = 0; e < kEach / 2; ++e) packed[e] = Pack<T>::pack(out[2 * e] * inv, out[2 * e + 1] * inv);
+        uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d0));
+#pragma unroll
+        for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
+        if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
+      } else {
+        const int64_t at_row = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) p.acc[at_row * D + d0 + e] = out[e];
+        if (d0 == 0) p.ml[at_row] = make_float2(top, sum);
+      }
+    }
+    if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
+      const int64_t last = at + w.s.tiles - 1;
+      int64_t n = (last - (range.end - 1) + range.total / range.n_cta - 1) / max(range.total / range.n_cta, (int64_t)1);
+      // ranges differ by one tile at most: correct the estimate
+      auto begin_of = [&](int64_t i) { return range.total / range.n_cta * i + range.total % range.n_cta * i / range.n_cta; };
+      while (n > 1 && begin_of(blockIdx.x + n) > last) --n;
+      while (begin_of(blockIdx.x + n + 1) <= last) ++n;
+      part = make_int2(w.b * units + w.unit, (int)n + 1);
+    }
+    at += w.t1 - w.t0;
+    going = w.next(p, units);
+  }
+  if (tid == 0) p.parts[blockIdx.x] = part;
+}
+
+// Joins the parts of the units that several CTAs hold.  Grid: (CTA in which the unit begins, query row).
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ float s_acc[kWarps][D];
+  __shared__ float s_sum[kWarps];
+  grid_before();
+  const int2 part = p.parts[blockIdx.x];
+  const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
+  const int r = blockIdx.y, b = part.x / units, u = part.x - b * units, h = u / query_blocks, row = (u - h * query_blocks) * kQ + r;
+  if (part.y < 2 || row >= p.G) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  auto place = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
+  float top = -INFINITY;
+  for (int i = lane; i < part.y; i += 32) top = fmaxf(top, p.ml[place(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  constexpr int kEach = D / 32;
+  float sum = 0.f, out[kEach] = {};
+#pragma unroll 4
+  for (int i = warp; i < part.y; i += kWarps) {
+    const float2 ml = p.ml[place(i)];
+    const float weight = fast_exp2(ml.x - base);
+    sum = fmaf(ml.y, weight, sum);
+    const float* x = p.acc + place(i) * D + lane * kEach;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[e] = fmaf(x[e], weight, out[e]);
+  }
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) s_acc[warp][lane * kEach + e] = out[e];
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) sum += s_sum[i];
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int d = threadIdx.x; d < D / 2; d += kThreads) {
+    float x = 0.f, y = 0.f;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) { x += s_acc[i][2 * d]; y += s_acc[i][2 * d + 1]; }
+    reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * p.o.off(b, row, h))[d] = Pack<T>::pack(x * inv, y * inv);
+  }
+  if (threadIdx.x == 0) p.lse[((int64_t)b * p.G + row) * p.H + h] = top + log2f(sum);
+}
+
+}  // namespace paged
+}  // namespace moda

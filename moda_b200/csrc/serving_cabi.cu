@@ -1,0 +1,267 @@
+// C ABI of the operators that serve token by token: rotary positions, the paged KV cache's append, and the
+// attention of one new token.  Declarations are in include/moda_b200.h.
+#include "../../include/moda_b200.h"
+
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "cabi_common.cuh"
+#include "profiler.cuh"
+#include "rotary_kernels.cuh"
+#include "paged_decode_kernel.cuh"
+
+namespace {
+
+using namespace moda;
+
+// The sizes that the three operators share.
+int check_sizes(const moda_problem* pr) {
+  if (pr == nullptr) return MODA_ERR_NULL;
+  if (pr->B < 1 || pr->T_kv < 1 || pr->H < 1 || pr->G < 1 || pr->L < 0) return MODA_ERR_SHAPE;
+  if (pr->B > 65535 || pr->H > 65535 || pr->G > 65535) return MODA_ERR_SHAPE;
+  if ((int64_t)pr->B * pr->T_kv > 0x7fffffff || (int64_t)pr->T_kv * pr->G > (int64_t)1 << 30) return MODA_ERR_SHAPE;
+  if ((int64_t)pr->H * (pr->G + 1) > 1 << 24) return MODA_ERR_SHAPE;
+  if (pr->D != 64 && pr->D != 128) return MODA_ERR_HEAD_DIM;
+  if (pr->dtype != MODA_BF16 && pr->dtype != MODA_FP16) return MODA_ERR_DTYPE;
+  return MODA_OK;
+}
+// rot may be NULL (no rotation) unless `required`.
+int check_rotary(const moda_rotary* rot, bool required, int D, rotary::Args* out) {
+  *out = rotary::Args{nullptr, 0, 0, 0, 1.f};
+  if (rot == nullptr) return required ? MODA_ERR_NULL : MODA_OK;
+  if (rot->inv_freq == nullptr) return MODA_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(rot->inv_freq) & 7u) return MODA_ERR_ALIGNMENT;
+  if (rot->rotary_dim < 16 || rot->rotary_dim > D || rot->rotary_dim % 16 != 0) return MODA_ERR_SHAPE;
+  *out = rotary::Args{rot->inv_freq, rot->rotary_dim, rot->interleaved != 0, 0, rot->scale};
+  return MODA_OK;
+}
+int check_pages(const moda_problem* pr, const moda_paged_cache* c, paged::Pages* out) {
+  if (c == nullptr || c->block_table == nullptr || c->seq_lens == nullptr) return MODA_ERR_NULL;
+  if (c->num_pages < 1 || c->page_size < 1 || c->max_pages < 1 || c->table_stride < 0) return MODA_ERR_SHAPE;
+  if ((reinterpret_cast<uintptr_t>(c->block_table) | reinterpret_cast<uintptr_t>(c->seq_lens)) & 3u) return MODA_ERR_ALIGNMENT;
+  if (int rc = check_tensor(&c->k, true, c->num_pages, c->page_size, pr->H)) return rc;
+  if (int rc = check_tensor(&c->v, true, c->num_pages, c->page_size, pr->H)) return rc;
+  out->k = to_view(&c->k); out->v = to_view(&c->v);
+  out->table = c->block_table; out->table_stride = c->table_stride; out->seq_lens = c->seq_lens;
+  out->num_pages = c->num_pages; out->page_size = c->page_size; out->max_pages = c->max_pages;
+  out->by_page = rotary::FastDiv((uint32_t)c->page_size);
+  return MODA_OK;
+}
+
+// Grid of the kernels that give a token to a warp: (tokens, shares of its vectors).  A token whose vectors one warp
+// can walk in a few steps stays whole (the sines are computed once); few tokens are shared by more warps, down to one
+// step of kBatch vectors a lane, until there are some 16 warps for each SM.
+dim3 token_grid(int64_t tokens, int vectors, int D, int n_sm, int* per_warp) {
+  const int lanes = 32 / (D / 16), step = lanes * rotary::kBatch, warps = rotary::kThreads / 32;
+  const int most = (vectors + step - 1) / step;
+  const int64_t shares = std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)n_sm * 16 / std::max<int64_t>(tokens, 1)));
+  const int steps = (int)((most + shares - 1) / shares);
+  *per_warp = steps * step;
+  const int64_t blocks = (tokens + warps - 1) / warps;
+  return dim3((unsigned)std::min<int64_t>(blocks, (int64_t)n_sm * 64), (unsigned)((vectors + *per_warp - 1) / *per_warp));
+}
+
+template <typename T, int D> void launch_rotary(const rotary::RotaryParams& p, dim3 grid, cudaStream_t st) {
+  rotary::rotary_kernel<T, D><<<grid, rotary::kThreads, 0, st>>>(p);
+}
+template <typename T, int D> void launch_append(const paged::AppendParams& p, dim3 grid, cudaStream_t st) {
+  paged::append_kernel<T, D><<<grid, rotary::kThreads, 0, st>>>(p);
+}
+
+int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v, const paged::Pages& pages, const int32_t* lengths,
+           const rotary::Args& rot, const moda_tensor4* k_copy, const moda_tensor4* v_copy, int n_sm, cudaStream_t st) {
+  paged::AppendParams p{};
+  p.k_copy = to_view(k_copy); p.v_copy = to_view(v_copy);
+  p.k = to_view(k); p.v = to_view(v); p.pages = pages; p.lengths = lengths; p.rot = rot;
+  p.B = pr->B; p.T = pr->T_kv; p.H = pr->H; p.by_t = rotary::FastDiv((uint32_t)pr->T_kv);
+  const dim3 grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm, &p.per_warp);
+  {
+    prof::Scope ps(prof::kPagedAppend, st);
+    const bool bf = pr->dtype == MODA_BF16;
+    if (pr->D == 128) bf ? launch_append<__nv_bfloat16, 128>(p, grid, st) : launch_append<__half, 128>(p, grid, st);
+    else bf ? launch_append<__nv_bfloat16, 64>(p, grid, st) : launch_append<__half, 64>(p, grid, st);
+  }
+  MODA_CUDA(cudaGetLastError());
+  g_last_launches += 1;
+  return MODA_OK;
+}
+
+int decode_ctas(int n_sm) { return 2 * n_sm; }
+// Scratch: which units are shared, their parts' maxima and sums, their parts.
+size_t parts_bytes(int n) { return ((size_t)n * sizeof(int2) + 255) & ~(size_t)255; }
+size_t ml_bytes(int n) { return (size_t)n * 2 * paged::kQ * sizeof(float2); }
+size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * 2 * paged::kQ * D * sizeof(float); }
+
+template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, cudaStream_t st) {
+  auto kern = paged::decode_kernel<T, D>;
+  constexpr size_t smem = paged::smem_bytes<D>();
+  if (int rc = opt_in_smem(kern, smem)) return rc;
+  {
+    prof::Scope ps(prof::kPagedDecode, st);
+    kern<<<n_cta, paged::kThreads, smem, st>>>(p);
+  }
+  MODA_CUDA(cudaGetLastError());
+  g_last_launches += 1;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n_cta, std::min(p.G, paged::kQ));
+  cfg.blockDim = dim3(paged::kThreads);
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e;
+  {
+    prof::Scope ps(prof::kPagedJoin, st);
+    e = cudaLaunchKernelEx(&cfg, paged::join_kernel<T, D>, p);
+  }
+  MODA_CUDA(e);
+  g_last_launches += 1;
+  return MODA_OK;
+}
+
+}  // namespace
+
+namespace moda {
+// The word of the paged kernels (paged::g_wrong) of the current device: read, and cleared when set.
+int read_paged_status(int* out) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, paged::g_wrong, sizeof(int));
+  if (e == cudaSuccess && v != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(paged::g_wrong, &zero, sizeof(int));
+  }
+  *out = v;
+  return (int)e;
+}
+}  // namespace moda
+
+extern "C" {
+
+int moda_b200_rotary(const moda_problem* prob, const moda_rotary* rot, const moda_positions* positions, int inverse,
+                     const moda_tensor4* q, const moda_tensor4* k, const moda_tensor4* q_out, const moda_tensor4* k_out, void* stream) {
+  if (int rc = check_sizes(prob)) return rc;
+  const int64_t B = prob->B, T = prob->T_kv, H = prob->H;
+  const bool has_k = k != nullptr && k->data != nullptr;
+  if (int rc = check_tensor(q, true, B, T * prob->G, H)) return rc;
+  if (int rc = check_tensor(k, false, B, T, H)) return rc;
+  if (int rc = check_tensor(q_out, true, B, T * prob->G, H)) return rc;
+  if (int rc = check_tensor(k_out, has_k, B, T, H)) return rc;
+  rotary::RotaryParams p{};
+  if (int rc = check_rotary(rot, true, prob->D, &p.rot)) return rc;
+  p.rot.inverse = inverse != 0;
+  if (positions != nullptr) {
+    if (reinterpret_cast<uintptr_t>(positions->data) & (positions->is_int64 ? 7u : 3u)) return MODA_ERR_ALIGNMENT;
+    p.pos = rotary::Positions{positions->data, positions->stride_b, positions->stride_t, positions->offset, positions->is_int64 != 0};
+  }
+  p.q = to_view(q); p.k = to_view(has_k ? k : nullptr); p.q_out = to_view(q_out); p.k_out = to_view(has_k ? k_out : nullptr);
+  p.B = prob->B; p.T = prob->T_kv; p.H = prob->H; p.G = prob->G;
+  p.vectors = prob->H * (prob->G + (has_k ? 1 : 0));
+  p.by_h = rotary::FastDiv((uint32_t)prob->H); p.by_t = rotary::FastDiv((uint32_t)prob->T_kv);
+  DeviceGuard guard(prob->device);
+  if (!guard.ok) return cuda_fail(guard.err);
+  g_last_launches = 0;
+  const int n_sm = sm_count(prob->device);
+  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const dim3 grid = token_grid(B * T, p.vectors, prob->D, n_sm, &p.per_warp);
+  {
+    prof::Scope ps(prof::kRotary, st);
+    const bool bf = prob->dtype == MODA_BF16;
+    if (prob->D == 128) bf ? launch_rotary<__nv_bfloat16, 128>(p, grid, st) : launch_rotary<__half, 128>(p, grid, st);
+    else bf ? launch_rotary<__nv_bfloat16, 64>(p, grid, st) : launch_rotary<__half, 64>(p, grid, st);
+  }
+  MODA_CUDA(cudaGetLastError());
+  g_last_launches += 1;
+  return MODA_OK;
+}
+
+int moda_b200_paged_append(const moda_problem* prob, const moda_tensor4* k, const moda_tensor4* v, const moda_paged_cache* cache,
+                           const int32_t* lengths, const moda_rotary* rot, void* stream) {
+  if (int rc = check_sizes(prob)) return rc;
+  if (int rc = check_tensor(k, true, prob->B, prob->T_kv, prob->H)) return rc;
+  if (int rc = check_tensor(v, true, prob->B, prob->T_kv, prob->H)) return rc;
+  if (reinterpret_cast<uintptr_t>(lengths) & 3u) return MODA_ERR_ALIGNMENT;
+  paged::Pages pages;
+  rotary::Args turn;
+  if (int rc = check_pages(prob, cache, &pages)) return rc;
+  if (int rc = check_rotary(rot, false, prob->D, &turn)) return rc;
+  DeviceGuard guard(prob->device);
+  if (!guard.ok) return cuda_fail(guard.err);
+  g_last_launches = 0;
+  const int n_sm = sm_count(prob->device);
+  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
+  return append(prob, k, v, pages, lengths, turn, nullptr, nullptr, n_sm, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, size_t* bytes) {
+  if (bytes == nullptr) return MODA_ERR_NULL;
+  if (int rc = check_sizes(prob)) return rc;
+  const int n_sm = sm_count(prob->device);
+  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
+  *bytes = decode_scratch(decode_ctas(n_sm), prob->D);
+  return MODA_OK;
+}
+
+int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, const moda_paged_cache* cache, const moda_tensor4* k,
+                           const moda_tensor4* v, const moda_tensor4* k_copy, const moda_tensor4* v_copy, const moda_depth_rows* depth,
+                           const moda_rotary* rot, const moda_tensor4* o, float* lse, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (int rc = check_sizes(prob)) return rc;
+  if (prob->T_kv != 1 || !(prob->scale == prob->scale)) return MODA_ERR_SHAPE;
+  const int64_t B = prob->B, H = prob->H, query_blocks = (prob->G + paged::kQ - 1) / paged::kQ;
+  if (B * H * query_blocks > 0x7fffffff) return MODA_ERR_SHAPE;
+  if (int rc = check_tensor(q, true, B, prob->G, H)) return rc;
+  if (int rc = check_tensor(o, true, B, prob->G, H)) return rc;
+  const bool own_key = k != nullptr && k->data != nullptr;
+  if (int rc = check_tensor(k, false, B, 1, H)) return rc;
+  if (int rc = check_tensor(v, own_key, B, 1, H)) return rc;
+  if (k_copy != nullptr && !own_key) return MODA_ERR_NULL;
+  if (int rc = check_tensor(k_copy, false, B, 1, H)) return rc;
+  if (int rc = check_tensor(v_copy, k_copy != nullptr && k_copy->data != nullptr, B, 1, H)) return rc;
+  if (lse == nullptr) return MODA_ERR_NULL;
+  if (reinterpret_cast<uintptr_t>(lse) & 3u) return MODA_ERR_ALIGNMENT;
+  paged::DecodeParams p{};
+  if (int rc = check_pages(prob, cache, &p.pages)) return rc;
+  if (int rc = check_rotary(rot, false, prob->D, &p.rot)) return rc;
+  if (depth != nullptr && prob->L > 0) {
+    const int64_t P = depth->positions_per_sequence;
+    if (P < 1 || P * prob->L > (int64_t)1 << 30) return MODA_ERR_SHAPE;
+    if (int rc = check_tensor(&depth->k, true, B, prob->L, H)) return rc;
+    if (int rc = check_tensor(&depth->v, true, B, prob->L, H)) return rc;
+    if (P > 1 && (depth->k_stride_position <= 0 || depth->k_stride_position % 8 || depth->v_stride_position <= 0 || depth->v_stride_position % 8))
+      return MODA_ERR_ALIGNMENT;
+    if (reinterpret_cast<uintptr_t>(depth->positions_seen) & 3u) return MODA_ERR_ALIGNMENT;
+    p.kd = to_view(&depth->k); p.vd = to_view(&depth->v);
+    p.kd_sp = depth->k_stride_position; p.vd_sp = depth->v_stride_position;
+    p.depth_positions = depth->positions_seen; p.P = (int)P; p.L = prob->L;
+    p.by_L = rotary::FastDiv((uint32_t)prob->L);
+  } else if (prob->L > 0) {
+    return MODA_ERR_NULL;
+  }
+  DeviceGuard guard(prob->device);
+  if (!guard.ok) return cuda_fail(guard.err);
+  const int n_sm = sm_count(prob->device);
+  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
+  const int n_cta = decode_ctas(n_sm);
+  if (workspace == nullptr || workspace_bytes < decode_scratch(n_cta, prob->D)) return MODA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
+  unsigned char* ws = static_cast<unsigned char*>(workspace);
+  p.q = to_view(q); p.o = to_view(o); p.lse = lse;
+  p.B = prob->B; p.H = prob->H; p.G = prob->G; p.own_key = own_key;
+  p.scale_log2 = prob->scale * 1.4426950408889634f;
+  p.parts = reinterpret_cast<int2*>(ws);
+  p.ml = reinterpret_cast<float2*>(ws + parts_bytes(n_cta));
+  p.acc = reinterpret_cast<float*>(ws + parts_bytes(n_cta) + ml_bytes(n_cta));
+  g_last_launches = 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (own_key)
+    if (int rc = append(prob, k, v, p.pages, nullptr, p.rot, k_copy, v_copy, n_sm, st)) return rc;
+  const bool bf = prob->dtype == MODA_BF16;
+  if (prob->D == 128) return bf ? decode<__nv_bfloat16, 128>(p, n_cta, st) : decode<__half, 128>(p, n_cta, st);
+  return bf ? decode<__nv_bfloat16, 64>(p, n_cta, st) : decode<__half, 64>(p, n_cta, st);
+}
+
+}  // extern "C"

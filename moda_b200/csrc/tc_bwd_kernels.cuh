@@ -79,8 +79,6 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 //                 statistics and only then lets dk/dv begin, so that whoever begins later may read
 //                 them too; dk/dv and the depth gradients call it last, so that a grid never
 //                 ends before the ones that were launched ahead of it.
-__device__ __forceinline__ void grid_started() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void grid_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ------------------------------------------------------------------ statistics pass
 // delta = rowsum(o * dO) from the stored o, and lse, both transposed to [B, H, T_qp] so that the

@@ -14,6 +14,7 @@
 //   forward(q, k, v, cached_k, cached_v, scale, G, mode, chunk_rows)
 //   backward(q, k, v, cached_k, cached_v, o, lse, dout, scale, G, mode, chunk_rows)
 //   cache_state([grad_k, grad_v]), cache_grads(state), cache_append(...), cache_attention(...): DepthKVCache
+//   rotary(...), paged_append(...), paged_decode(...): rotary positions, paged KV cache
 //   set_path(path), set_check(fn)
 #include <Python.h>
 
@@ -302,6 +303,175 @@ Out attention(const Op& op, const Tensor& q, const Tensor& k, const Tensor& v, c
   return r;
 }
 
+// ------------------------------------------------------------------ rotary positions, paged KV cache
+// Raises AssertionError, as the Python wrappers' checks of shapes do.
+void require(bool ok, const char* what) {
+  if (ok) return;
+  PyGILState_STATE gil = PyGILState_Ensure();
+  PyErr_SetString(PyExc_AssertionError, what);
+  python_error err;
+  err.persist();
+  PyGILState_Release(gil);
+  throw err;
+}
+void require_type(bool ok, const char* what) { TORCH_CHECK_TYPE(ok, what); }
+
+struct RotarySpec {                   // moda_b200.Rotary
+  Tensor inv_freq;
+  bool interleaved = false;
+  double scale = 1.;
+  moda_rotary abi() const {
+    return moda_rotary{inv_freq.const_data_ptr<double>(), (int32_t)(2 * inv_freq.numel()), interleaved ? 1 : 0, (float)scale};
+  }
+};
+RotarySpec as_rotary(PyObject* x, const Tensor& like) {
+  RotarySpec r;
+  require_type(PyTuple_Check(x) && PyTuple_GET_SIZE(x) == 3 && THPVariable_Check(PyTuple_GET_ITEM(x, 0)), "moda_b200: rotary must be a moda_b200.Rotary");
+  r.inv_freq = THPVariable_Unpack(PyTuple_GET_ITEM(x, 0));
+  r.interleaved = PyObject_IsTrue(PyTuple_GET_ITEM(x, 1)) == 1;
+  r.scale = PyFloat_AsDouble(PyTuple_GET_ITEM(x, 2));
+  if (r.scale == -1. && PyErr_Occurred()) throw python_error();
+  require_type(r.inv_freq.scalar_type() == at::kDouble, "moda_b200: inv_freq must be float64");
+  require(r.inv_freq.dim() == 1 && r.inv_freq.is_contiguous(), "inv_freq must be a contiguous vector");
+  require(r.inv_freq.numel() > 0 && r.inv_freq.numel() % 8 == 0 && 2 * r.inv_freq.numel() <= like.size(-1),
+          "inv_freq must hold rotary_dim / 2 frequencies, with rotary_dim a multiple of 16 of at most head_dim");
+  require(r.inv_freq.device() == like.device(), "all tensors must be on one device");
+  TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && r.inv_freq.requires_grad()), "moda_b200: no gradient with regard to inv_freq");
+  return r;
+}
+// The checks that every operator's data tensors go through; the last, so that shapes are looked at without a GPU too.
+void require_data(std::initializer_list<const Tensor*> xs, const Tensor& q) {
+  TORCH_CHECK(q.is_cuda(), "moda_b200 runs on CUDA tensors only (there is no CPU path)");
+  require_type(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, "moda_b200 supports bf16/fp16 inputs");
+  for (const Tensor* x : xs)
+    require(!x->defined() || (x->scalar_type() == q.scalar_type() && x->device() == q.device()), "all tensors must share dtype and device");
+}
+moda_problem serving_problem(const Tensor& rows, int64_t T, int64_t G, double scale) {
+  moda_problem pr{};
+  pr.B = (int32_t)rows.size(0);
+  pr.T_kv = (int32_t)T;
+  pr.H = (int32_t)rows.size(2);
+  pr.D = (int32_t)rows.size(3);
+  pr.G = (int32_t)G;
+  pr.dtype = rows.scalar_type() == at::kBFloat16 ? MODA_BF16 : MODA_FP16;
+  pr.scale = (float)scale;
+  pr.device = rows.get_device();
+  return pr;
+}
+// The kernels index a tensor's rows and pages with the extents of the problem, in 32 bits.
+void require_sizes(std::initializer_list<int64_t> xs) {
+  for (int64_t x : xs) require(x <= 0x7fffffff, "a size exceeds 2^31 - 1");
+}
+
+struct RotaryOp {
+  RotarySpec spec;
+  int64_t G = 1, offset = 0;
+  bool inverse = false;
+};
+Tensor turned(const RotaryOp& op, const Tensor& q_, const Tensor& k_, const Tensor& positions, int64_t G, Tensor* k_out) {
+  const Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_);
+  const int64_t T = q.size(1) / G;
+  const moda_problem pr = serving_problem(q, T, G, 1.);
+  const moda_rotary rot = op.spec.abi();
+  moda_positions pos{};
+  pos.offset = op.offset;
+  if (positions.defined()) {
+    pos.data = positions.const_data_ptr();
+    pos.stride_t = T > 1 ? positions.stride(-1) : 0;
+    pos.stride_b = positions.dim() == 2 && positions.size(0) > 1 ? positions.stride(0) : 0;
+    pos.is_int64 = positions.scalar_type() == at::kLong;
+  }
+  const Tensor q_out = at::empty(q.sizes(), q.options());
+  if (k.defined()) *k_out = at::empty(k.sizes(), k.options());
+  const c10::cuda::CUDAGuard guard(q.device());
+  check_status(moda_b200_rotary(&pr, &rot, &pos, op.inverse, T4(q).p(), T4(k).p(), T4(q_out).p(), T4(*k_out).p(),
+                                c10::cuda::getCurrentCUDAStream().stream()),
+               "moda_b200_rotary");
+  return q_out;
+}
+struct Pair { Tensor q, k; };
+Pair rotary(const RotaryOp& op, const Tensor& q, const Tensor& k, const Tensor& positions);
+
+// The transposed map is the rotation by the negative angles, which is the same operator (and has a derivative of its own).
+struct MoDARotaryBackward : public Node {
+  RotaryOp op;
+  SavedVariable positions;
+  at::ScalarType dtype = at::kBFloat16;
+  std::string name() const override { return "MoDARotaryBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    positions.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(next_edges().size());
+    std::unique_lock<std::mutex> lock(mutex_);
+    const Tensor at = positions.unpack();
+    lock.unlock();
+    auto typed = [&](const Tensor& x) { return x.scalar_type() == dtype ? x : x.to(dtype); };
+    RotaryOp back = op;
+    back.inverse = !op.inverse;
+    const bool with_q = grads[0].defined() && task_should_compute_output(0);
+    const bool with_k = grads.size() > 1 && grads[1].defined() && task_should_compute_output(1);
+    if (with_q) {
+      Pair r = rotary(back, typed(grads[0]), with_k ? typed(grads[1]) : Tensor(), at);
+      out[0] = std::move(r.q);
+      if (with_k) out[1] = std::move(r.k);
+    } else if (with_k) {
+      back.G = 1;
+      out[1] = rotary(back, typed(grads[1]), Tensor(), at).q;
+    }
+    return out;
+  }
+};
+Pair rotary(const RotaryOp& op, const Tensor& q, const Tensor& k, const Tensor& positions) {
+  refuse_tangents({&q, &k});
+  const bool grad = wants_grad({&q, &k});
+  Pair r;
+  {
+    at::AutoGradMode no_grad(false);
+    r.q = turned(op, q, k, positions, op.G, &r.k);
+  }
+  if (!grad) return r;
+  std::shared_ptr<MoDARotaryBackward> node(new MoDARotaryBackward(), torch::autograd::deleteNode);
+  node->op = op;
+  node->dtype = q.scalar_type();
+  node->positions = SavedVariable(positions, false);
+  node->set_next_edges(torch::autograd::collect_next_edges(q, k));
+  torch::autograd::set_history(r.q, node);
+  if (k.defined()) torch::autograd::set_history(r.k, node);
+  return r;
+}
+
+struct PagedCache {                   // cache_k, cache_v, block_table, seq_lens as arguments a[0] .. a[3]
+  Tensor k, v, table, lens;
+  moda_paged_cache abi{};
+};
+PagedCache as_paged(PyObject* const* a, int64_t B, int64_t H, int64_t D) {
+  PagedCache c;
+  for (int i = 0; i < 4; ++i) require_type(THPVariable_Check(a[i]), "moda_b200: the cache, its block table and seq_lens must be tensors");
+  c.k = THPVariable_Unpack(a[0]); c.v = THPVariable_Unpack(a[1]); c.table = THPVariable_Unpack(a[2]); c.lens = THPVariable_Unpack(a[3]);
+  require(c.k.dim() == 4 && c.k.size(2) == H && c.k.size(3) == D, "cache_k must be [num_pages, page_size, H, D] with the H and D of the call");
+  require(c.v.sizes() == c.k.sizes(), "cache_v must have the shape of cache_k");
+  require(c.k.numel() > 0, "the cache has no pages");
+  require(usable(c.k) && usable(c.v), "the cache is used in place: its innermost stride must be 1, the others positive multiples of 8, and it "
+                                      "must start on a 16-byte boundary");
+  require_type(c.table.scalar_type() == at::kInt && c.lens.scalar_type() == at::kInt, "moda_b200: block_table and seq_lens must be int32");
+  require(c.table.dim() == 2 && c.table.size(0) == B && c.table.size(1) > 0 && (c.table.size(1) == 1 || c.table.stride(1) == 1) && c.table.stride(0) >= 0,
+          "block_table must be [B, max_pages], with the pages of a sequence one after another");
+  require(c.lens.dim() == 1 && c.lens.size(0) == B && c.lens.is_contiguous(), "seq_lens must be [B], contiguous");
+  require_sizes({c.k.size(0), c.k.size(1), c.table.size(1)});
+  require(c.table.device() == c.k.device() && c.lens.device() == c.k.device(), "all tensors must be on one device");
+  c.abi.k = T4(c.k).t; c.abi.v = T4(c.v).t;
+  c.abi.num_pages = (int32_t)c.k.size(0); c.abi.page_size = (int32_t)c.k.size(1);
+  c.abi.block_table = c.table.const_data_ptr<int32_t>(); c.abi.table_stride = c.table.stride(0); c.abi.max_pages = (int32_t)c.table.size(1);
+  c.abi.seq_lens = c.lens.const_data_ptr<int32_t>();
+  return c;
+}
+void refuse_gradients(std::initializer_list<const Tensor*> xs) {
+  TORCH_CHECK(!wants_grad(xs), "moda_b200: the paged cache serves and does not train: call it under torch.no_grad()");
+  refuse_tangents(xs);
+}
+
 // ------------------------------------------------------------------ Python side
 struct NoGil {                        // ctypes dropped the interpreter lock around the library call; so does this
   PyThreadState* s = PyEval_SaveThread();
@@ -521,6 +691,150 @@ PyObject* py_cache_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// rotary(q, k, rotary, positions, G) -> (q, k); positions: None, a tensor of whole numbers, or the first one
+PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 5)) return nullptr;
+  require_type(THPVariable_Check(a[0]) && tensor_or_none_check(a[1]), "moda_b200: the operands must be tensors");
+  const Tensor q = tensor_or_none(a[0]), k = tensor_or_none(a[1]);
+  RotaryOp op;
+  op.G = as_int(a[4]);
+  require(q.dim() == 4, "q must be [B, T * moda_group_num, H, D]");
+  require(op.G > 0 && q.size(1) % op.G == 0, "T_q must be divisible by moda_group_num");
+  const int64_t B = q.size(0), T = q.size(1) / op.G;
+  require(!k.defined() || (k.dim() == 4 && k.size(0) == B && k.size(1) == T && k.size(2) == q.size(2) && k.size(3) == q.size(3)),
+          "k must be [B, T, H, D] where q is [B, T * moda_group_num, H, D]");
+  op.spec = as_rotary(a[2], q);
+  Tensor positions;
+  if (THPVariable_Check(a[3])) {
+    positions = THPVariable_Unpack(a[3]);
+    require_type(positions.scalar_type() == at::kInt || positions.scalar_type() == at::kLong, "moda_b200: positions must be int32 or int64");
+    require((positions.dim() == 1 && positions.size(0) == T) || (positions.dim() == 2 && (positions.size(0) == B || positions.size(0) == 1) && positions.size(1) == T),
+            "positions must be [T] or [B, T]");
+    require(positions.device() == q.device(), "all tensors must be on one device");
+  } else if (a[3] != Py_None) {
+    op.offset = PyLong_AsLongLong(a[3]);
+    if (op.offset == -1 && PyErr_Occurred()) throw python_error();
+  }
+  require_data({&k}, q);
+  require_sizes({B, q.size(1), q.size(2), q.size(3)});
+  Pair r;
+  {
+    NoGil no_gil;
+    r = rotary(op, q, k, positions);
+  }
+  return wrap(Out{r.q, r.k});
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(k, v, cache_k, cache_v, block_table, seq_lens, lengths, rotary)
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 8)) return nullptr;
+  require_type(THPVariable_Check(a[0]) && THPVariable_Check(a[1]) && tensor_or_none_check(a[6]), "moda_b200: the operands must be tensors");
+  const Tensor k_ = tensor_or_none(a[0]), v_ = tensor_or_none(a[1]), lengths = tensor_or_none(a[6]);
+  require(k_.dim() == 4 && v_.sizes() == k_.sizes(), "k and v must be [B, T, H, D]");
+  const int64_t B = k_.size(0);
+  const PagedCache c = as_paged(a + 2, B, k_.size(2), k_.size(3));
+  if (lengths.defined()) {
+    require_type(lengths.scalar_type() == at::kInt, "moda_b200: lengths must be int32");
+    require(lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous() && lengths.device() == k_.device(), "lengths must be [B], contiguous, on the tensors' device");
+  }
+  RotarySpec spec;
+  if (a[7] != Py_None) spec = as_rotary(a[7], k_);
+  require_data({&v_, &c.k, &c.v}, k_);
+  require_sizes({B, k_.size(1), k_.size(2), k_.size(3)});
+  {
+    NoGil no_gil;
+    refuse_gradients({&k_, &v_, &c.k, &c.v});
+    at::AutoGradMode no_grad(false);
+    const Tensor k = in_place_or_copy(k_), v = in_place_or_copy(v_);
+    const moda_problem pr = serving_problem(k, k.size(1), 1, 1.);
+    const moda_rotary rot = spec.inv_freq.defined() ? spec.abi() : moda_rotary{};
+    const c10::cuda::CUDAGuard guard(k.device());
+    check_status(moda_b200_paged_append(&pr, T4(k).p(), T4(v).p(), &c.abi, lengths.defined() ? lengths.const_data_ptr<int32_t>() : nullptr,
+                                        spec.inv_freq.defined() ? &rot : nullptr, c10::cuda::getCurrentCUDAStream().stream()),
+                 "moda_b200_paged_append");
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale, G, rotary, record_k, record_v) -> (o, lse)
+PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (!arg_count(n, 15)) return nullptr;
+  require_type(THPVariable_Check(a[0]), "moda_b200: the operands must be tensors");
+  for (int i : {5, 6, 7, 8, 9, 13, 14}) require_type(tensor_or_none_check(a[i]), "moda_b200: the operands must be tensors");
+  const Tensor q_ = tensor_or_none(a[0]), k_ = tensor_or_none(a[5]), v_ = tensor_or_none(a[6]), rk = tensor_or_none(a[13]), rv = tensor_or_none(a[14]);
+  const Tensor seen = tensor_or_none(a[9]);
+  Tensor ck_ = tensor_or_none(a[7]), cv_ = tensor_or_none(a[8]);
+  const int64_t G = as_int(a[11]);
+  require(q_.dim() == 4 && G > 0 && q_.size(1) == G, "q must be [B, moda_group_num, H, D]: one token of each sequence");
+  const int64_t B = q_.size(0), H = q_.size(2), D = q_.size(3);
+  const double scale = as_scale(a[10], q_);
+  const PagedCache c = as_paged(a + 1, B, H, D);
+  auto one_row = [&](const Tensor& x) { return x.dim() == 4 && x.size(0) == B && x.size(1) == 1 && x.size(2) == H && x.size(3) == D; };
+  require(k_.defined() == v_.defined(), "k and v must be given together");
+  require(!k_.defined() || (one_row(k_) && one_row(v_)), "k and v must be [B, 1, H, D]");
+  require(rk.defined() == rv.defined() && (!rk.defined() || k_.defined()), "record_k and record_v must be given together, and with k and v");
+  require(!rk.defined() || (one_row(rk) && one_row(rv) && usable(rk) && usable(rv)),
+          "record_k and record_v are written in place: [B, 1, H, D], innermost stride 1, the others positive multiples of 8, on a 16-byte boundary");
+  require(ck_.defined() == cv_.defined(), "cached_k and cached_v must be given together");
+  int64_t P = 1, L = 0;
+  if (ck_.defined()) {
+    require((ck_.dim() == 4 || ck_.dim() == 5) && cv_.sizes() == ck_.sizes() && ck_.size(0) == B && ck_.size(-2) == H && ck_.size(-1) == D,
+            "cached_k and cached_v must be [B, L, H, D], or [B, P, L, H, D] with depth_positions");
+    require((ck_.dim() == 5) == seen.defined(), "depth_positions belongs to depth rows of several positions, [B, P, L, H, D]");
+    if (ck_.dim() == 5) P = ck_.size(1);
+    L = ck_.size(-3);
+    require(P * L <= (int64_t)1 << 30, "too many depth rows");
+    if (P * L == 0) ck_ = cv_ = Tensor(), L = 0;
+  }
+  if (seen.defined()) {
+    require_type(seen.scalar_type() == at::kInt, "moda_b200: depth_positions must be int32");
+    require(seen.dim() == 1 && seen.size(0) == B && seen.is_contiguous() && seen.device() == q_.device() && a[7] != Py_None,
+            "depth_positions must be [B], contiguous, on the tensors' device, with cached_k and cached_v");
+  }
+  RotarySpec spec;
+  if (a[12] != Py_None) spec = as_rotary(a[12], q_);
+  require_data({&c.k, &c.v, &k_, &v_, &ck_, &cv_, &rk, &rv}, q_);
+  require_sizes({B, H, D});
+  Out r;
+  {
+    NoGil no_gil;
+    refuse_gradients({&q_, &k_, &v_, &c.k, &c.v, &ck_, &cv_});
+    at::AutoGradMode no_grad(false);
+    const Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_), ck = in_place_or_copy(ck_), cv = in_place_or_copy(cv_);
+    moda_problem pr = serving_problem(q, 1, G, scale);
+    pr.L = (int32_t)L;
+    const moda_rotary rot = spec.inv_freq.defined() ? spec.abi() : moda_rotary{};
+    moda_depth_rows depth{};
+    if (L > 0) {
+      auto rows = [](const Tensor& x) {
+        return moda_tensor4{const_cast<void*>(x.const_data_ptr()), x.stride(0), x.stride(-3), x.stride(-2)};
+      };
+      depth.k = rows(ck); depth.v = rows(cv);
+      depth.k_stride_position = ck.dim() == 5 ? ck.stride(1) : 0;
+      depth.v_stride_position = cv.dim() == 5 ? cv.stride(1) : 0;
+      depth.positions_per_sequence = (int32_t)P;
+      depth.positions_seen = seen.defined() ? seen.const_data_ptr<int32_t>() : nullptr;
+    }
+    const c10::cuda::CUDAGuard guard(q.device());
+    r.o = at::empty(q.sizes(), q.options());
+    r.lse = at::empty({B, G, H}, q.options().dtype(at::kFloat));
+    size_t bytes = 0;
+    check_status(moda_b200_paged_decode_workspace_bytes(&pr, &bytes), "moda_b200_paged_decode_workspace_bytes");
+    const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    check_status(moda_b200_paged_decode(&pr, T4(q).p(), &c.abi, T4(k).p(), T4(v).p(), T4(rk).p(), T4(rv).p(), L > 0 ? &depth : nullptr,
+                                        spec.inv_freq.defined() ? &rot : nullptr, T4(r.o).p(), r.lse.mutable_data_ptr<float>(),
+                                        ws.mutable_data_ptr(), bytes, c10::cuda::getCurrentCUDAStream().stream()),
+                 "moda_b200_paged_decode");
+  }
+  return wrap(r);
+  END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_set_path(PyObject*, PyObject* x) {
   const long v = PyLong_AsLong(x);
   if (v == -1 && PyErr_Occurred()) return nullptr;
@@ -541,6 +855,9 @@ PyMethodDef kMethods[] = {{"attention", MODA_FAST(py_attention), nullptr},
                           {"cache_grads", py_cache_grads, METH_O, nullptr},
                           {"cache_append", MODA_FAST(py_cache_append), nullptr},
                           {"cache_attention", MODA_FAST(py_cache_attention), nullptr},
+                          {"rotary", MODA_FAST(py_rotary), nullptr},
+                          {"paged_append", MODA_FAST(py_paged_append), nullptr},
+                          {"paged_decode", MODA_FAST(py_paged_decode), nullptr},
                           {"set_path", py_set_path, METH_O, nullptr},
                           {"set_check", py_set_check, METH_O, nullptr},
                           {nullptr, nullptr, 0, nullptr}};

@@ -1,0 +1,383 @@
+"""GPU: the paged KV cache's append and the attention of one new token, against plain forms in 64 bits."""
+import pytest
+import torch
+
+from tests.serving_reference import attend, attend_bounds, close, rows_of, turn, turn_bound
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _pool(gen, dtype, lens, room, page, H, D, heads=True, spare=3, fill=float("nan")):
+    """A pool in which every sequence has its own pages, in a random order, filled up to its length; the rest is `fill`."""
+    B = len(lens)
+    need = max(1, -(-(max(lens) + room) // page))
+    pages = B * need + spare
+    table = torch.randperm(pages, generator=gen, device=DEV)[: B * need].view(B, need).int()
+    caches = []
+    for _ in range(2):
+        x = torch.full((pages, H, page, D) if heads else (pages, page, H, D), fill, device=DEV, dtype=dtype)
+        x = x.transpose(1, 2) if heads else x
+        for b, n in enumerate(lens):
+            j = torch.arange(n, device=DEV)
+            x[table[b, j // page].long(), j % page] = torch.randn(n, H, D, generator=gen, device=DEV).to(dtype)
+        caches.append(x)
+    return caches, table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+def _rand(gen, dtype, *shape):
+    return torch.randn(*shape, generator=gen, device=DEV).to(dtype)
+
+
+def _check_decode(o, lse, q, caches, table, lens, scale, depth=None, turned=None, seen=None):
+    """turned: (rotary, positions).  Keys are taken from the cache as it is now."""
+    q64 = q.double()
+    if turned is not None:
+        rotary, at = turned
+        q64 = turn(q64, at[:, None], rotary.inv_freq, rotary.interleaved, rotary.scale)
+    for b, n in enumerate(lens):
+        keys, values = (rows_of(c, table[b], n).double() for c in caches)
+        if depth is not None:
+            kd, vd = (x[b].double() if seen is None else x[b, : int(seen[b])].flatten(0, 1).double() for x in depth)
+            keys, values = torch.cat([keys, kd]), torch.cat([values, vd])
+        want_o, want_lse, size, mass = attend(q64[b], keys, values, scale)
+        tol_o, tol_lse = attend_bounds(want_o, want_lse, size, mass, q.shape[-1], q.dtype, turned is not None)
+        close(o[b], want_o, tol_o, f"o of sequence {b}")
+        close(lse[b], want_lse, tol_lse, f"lse of sequence {b}")
+
+
+DECODE = [  # dtype, lengths, H, G, D, L, page, heads
+    (BF, [0], 1, 1, 64, 0, 1, True),
+    (BF, [1], 1, 1, 64, 0, 16, True),
+    (HF, [1, 0, 2], 2, 3, 128, 1, 5, False),
+    (BF, [16, 17, 15, 31], 3, 4, 128, 7, 16, True),
+    (HF, [256], 4, 1, 64, 4, 16, True),
+    (BF, [1000, 3, 0, 511, 64], 5, 8, 128, 11, 24, False),
+    (HF, [777, 778, 1, 65], 2, 9, 64, 3, 8, True),
+    (BF, [300, 40], 1, 20, 128, 0, 64, False),
+    (BF, [5000], 2, 4, 128, 32, 64, True),
+    (HF, [20000, 1], 1, 2, 64, 1, 128, True),
+    (BF, list(range(0, 290, 2)), 2, 2, 64, 5, 32, True),       # more sequences than a CTA has threads
+    (BF, [33], 200, 1, 64, 2, 256, False),
+]
+
+
+@pytest.mark.parametrize("dtype,lens,H,G,D,L,page,heads", DECODE)
+def test_decode(built_library, dtype, lens, H, G, D, L, page, heads):
+    """Rows behind a sequence's end, pages of nobody and whole unused pages hold NaN."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(len(lens) + H + L)
+    B = len(lens)
+    caches, table, n = _pool(gen, dtype, lens, 5, page, H, D, heads)
+    q = _rand(gen, dtype, B, G, H, D)
+    depth = tuple(_rand(gen, dtype, B, L, H, D) for _ in range(2)) if L else None
+    kw = dict(cached_k=depth[0], cached_v=depth[1]) if L else {}
+    o, lse = M.paged_moda_decode(q, *caches, table, n, **kw, moda_group_num=G, need_lse=True)
+    _check_decode(o, lse, q, caches, table, lens, D ** -0.5, depth)
+    again = M.paged_moda_decode(q, *caches, table, n, **kw, moda_group_num=G, need_lse=True)
+    assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+    assert M.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,lens,H,G,D,L,page,heads", DECODE)
+@pytest.mark.parametrize("interleaved,rot", [(False, 64), (True, 32)])
+def test_step(built_library, dtype, lens, H, G, D, L, page, heads, interleaved, rot):
+    """With the token's own key and value, turned, appended and recorded."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(len(lens) + H + L + 1)
+    B = len(lens)
+    caches, table, n = _pool(gen, dtype, lens, 1, page, H, D, heads)
+    before = [c.clone() for c in caches]
+    q, k, v = _rand(gen, dtype, B, G, H, D), _rand(gen, dtype, B, 1, H, D), _rand(gen, dtype, B, 1, H, D)
+    rotary = M.Rotary(M.rotary_frequencies(rot, device=DEV)[0], interleaved, 1.1)
+    depth = tuple(_rand(gen, dtype, B, L + 2, H, D) for _ in range(2))
+    kw = dict(cached_k=depth[0][:, :L], cached_v=depth[1][:, :L], record_k=depth[0][:, L : L + 1], record_v=depth[1][:, L : L + 1])
+    was = [x.clone() for x in depth]
+    o, lse = M.paged_moda_decode(q, *caches, table, n, k, v, **kw, rotary=rotary, moda_group_num=G, need_lse=True)
+    _check_decode(o, lse, q, caches, table, [x + 1 for x in lens], D ** -0.5, [x[:, :L] for x in depth] if L else None, (rotary, n.long()))
+    want = turn(k.double(), n.long()[:, None], rotary.inv_freq, interleaved, 1.1)
+    at = torch.arange(B, device=DEV)
+    pages, slots = table[at, n.long() // page].long(), n.long() % page
+    new_k, new_v = caches[0][pages, slots], caches[1][pages, slots]
+    close(new_k[:, None], want, turn_bound(k.double(), want, rot, interleaved, 1.1, dtype), "the key's row")
+    assert torch.equal(new_v[:, None], v)
+    assert torch.equal(depth[0][:, L], new_k) and torch.equal(depth[1][:, L], new_v)
+    for c, old, new in zip(caches, before, (new_k, new_v)):            # nothing else has been written
+        old[pages, slots] = new
+        assert torch.equal(c.view(torch.int16), old.view(torch.int16))
+    for x, old in zip(depth, was):
+        assert torch.equal(x[:, :L], old[:, :L]) and torch.equal(x[:, L + 1], old[:, L + 1])
+    assert n.tolist() == lens and M.device_status() == 0
+
+
+APPEND = [  # dtype, T, held, lengths, H, D, page, heads, rot, interleaved
+    (BF, 1, [0], [1], 1, 64, 1, True, 64, False),
+    (HF, 1, [5, 0, 64, 63], [1, 1, 1, 1], 8, 128, 64, True, 128, False),
+    (BF, 7, [3, 0, 11], [7, 0, 4], 3, 128, 5, False, 96, True),
+    (HF, 130, [0, 17], [130, 129], 2, 64, 16, True, 16, False),
+    (BF, 33, [1], None, 20, 64, 24, False, 0, False),
+    (BF, 1500, [0, 100, 7], [1500, 1, 777], 4, 128, 64, True, 64, True),
+    (HF, 2, list(range(150)), None, 1, 64, 8, True, 48, True),
+]
+
+
+@pytest.mark.parametrize("dtype,T,held,lengths,H,D,page,heads,rot,interleaved", APPEND)
+def test_append(built_library, dtype, T, held, lengths, H, D, page, heads, rot, interleaved):
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(T + H)
+    B = len(held)
+    caches, table, n = _pool(gen, dtype, held, T, page, H, D, heads)
+    before = [c.clone() for c in caches]
+    k, v = _rand(gen, dtype, B, T, H, D), _rand(gen, dtype, B, T, H, D)
+    count = torch.tensor(lengths if lengths is not None else [T] * B, dtype=torch.int32, device=DEV)
+    rotary = M.Rotary(M.rotary_frequencies(rot, device=DEV)[0], interleaved, 0.9) if rot else None
+    M.paged_moda_append(k, v, *caches, table, n, None if lengths is None else count, rotary)
+    assert M.last_launch_count() == 1
+    at = n.long()[:, None] + torch.arange(T, device=DEV)
+    want = turn(k.double(), at, rotary.inv_freq, interleaved, 0.9) if rot else k.double()
+    tol = turn_bound(k.double(), want, rot, interleaved, 0.9, dtype) if rot else torch.zeros_like(want)
+    for b in range(B):
+        j = at[b, : int(count[b])]
+        pages, slots = table[b, j // page].long(), j % page
+        close(caches[0][pages, slots], want[b, : len(j)], tol[b, : len(j)], "keys")
+        assert torch.equal(caches[1][pages, slots], v[b, : len(j)])
+        for c, old in zip(caches, before):
+            old[pages, slots] = c[pages, slots]
+    for c, old in zip(caches, before):                                  # nothing else has been written
+        assert torch.equal(c.view(torch.int16), old.view(torch.int16))
+    assert M.device_status() == 0
+
+
+def test_strides_scale_and_views(built_library):
+    """Caches that are slices of something larger, queries and rows that are views, shared pages, and scales of either sign."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    B, H, G, D, page, L = 3, 2, 4, 64, 16, 3
+    wide = torch.full((12, page, 2, H + 2, D + 8), float("nan"), device=DEV, dtype=BF)
+    caches = [wide[:, :, i, 1 : H + 1, :D] for i in range(2)]
+    lens = [70, 33, 16]
+    table = torch.tensor([[0, 7, 3, 9, 1], [0, 7, 4, 11, 11], [0, 5, 5, 5, 5]], device=DEV, dtype=torch.int32)       # a common first page
+    for c in caches:
+        c.copy_(torch.randn(c.shape, generator=gen, device=DEV))
+    wide_table = torch.zeros(B, 8, dtype=torch.int32, device=DEV)
+    wide_table[:, 2:7] = table
+    q = _rand(gen, BF, B, 2 * G, H + 1, D)[:, ::2, 1:]
+    depth = [_rand(gen, BF, B, 5, 9, H, D).permute(0, 2, 1, 3, 4)[:, 1:3, :L] for _ in range(2)]
+    n, seen = torch.tensor(lens, dtype=torch.int32, device=DEV), torch.tensor([2, 0, 1], dtype=torch.int32, device=DEV)
+    for scale in (0.3, -0.2, 0.0, 4.0):
+        o, lse = M.paged_moda_decode(q, *caches, wide_table[:, 2:7], n, cached_k=depth[0], cached_v=depth[1], depth_positions=seen,
+                                     scale=scale, moda_group_num=G, need_lse=True)
+        _check_decode(o, lse, q, caches, table, lens, scale, depth, seen=seen)
+    odd = _rand(gen, BF, B, G, H, D + 1)[..., 1:]                       # not on a 16-byte boundary: copied
+    o, lse = M.paged_moda_decode(odd, *caches, table, n, moda_group_num=G, need_lse=True)
+    _check_decode(o, lse, odd, caches, table, lens, D ** -0.5)
+
+
+def test_large_scores(built_library):
+    """Scores of some hundreds, in growing and in falling order: the running maximum moves at every tile, or once."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(10)
+    n, H, G, D, page = 700, 2, 2, 64, 32
+    for order in (1, -1):
+        caches, table, lens = _pool(gen, BF, [n], 0, page, H, D)
+        q = torch.ones(1, G, H, D, device=DEV, dtype=BF)
+        j = torch.arange(n, device=DEV)
+        caches[0][table[0, j // page].long(), j % page] = (order * (j - n / 2) / 8).bfloat16()[:, None, None].expand(n, H, D)
+        o, lse = M.paged_moda_decode(q, *caches, table, lens, moda_group_num=G, need_lse=True)
+        _check_decode(o, lse, q, caches, table, [n], D ** -0.5)
+
+
+def test_nan_stays_where_it_belongs(built_library):
+    """A NaN key of one sequence's head spoils that head's result and no other."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    lens = [40, 40]
+    caches, table, n = _pool(gen, HF, lens, 0, 16, 2, 64)
+    caches[0][table[0, 1].long(), 3, 1] = float("nan")
+    q = _rand(gen, HF, 2, 2, 2, 64)
+    o, lse = M.paged_moda_decode(q, *caches, table, n, moda_group_num=2, need_lse=True)
+    assert o[0, :, 1].isnan().all() and lse[0, :, 1].isnan().all()
+    assert not o[0, :, 0].isnan().any() and not o[1].isnan().any() and not lse[1].isnan().any()
+
+
+def test_bad_tables_and_lengths_are_left_out_and_recorded(built_library):
+    """Page numbers outside the pool: the kernels look at each before they use it.  Lengths outside the table: bounded by it."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(12)
+    H, G, D, page = 2, 2, 64, 16
+    lens = [60, 50]
+    caches, table, n = _pool(gen, BF, lens, 4, page, H, D)
+    q = _rand(gen, BF, 2, G, H, D)
+    pages = caches[0].shape[0]
+    for bad in (-1, pages, 2 ** 31 - 1, -2 ** 31):
+        broken = table.clone()
+        broken[0, 1] = bad
+        o, lse = M.paged_moda_decode(q, *caches, broken, n, moda_group_num=G, need_lse=True)
+        assert M.device_status() == (2 << 8 | 1) and M.device_status() == 0
+        keep = [j for j in range(60) if j // page != 1]
+        keys, values = (rows_of(c, table[0], 60)[keep].double() for c in caches)
+        want = attend(q[0].double(), keys, values, D ** -0.5)
+        tol = attend_bounds(*want, D, BF, False)
+        close(o[0], want[0], tol[0], "o"), close(lse[0], want[1], tol[1], "lse")
+        _check_decode(o[1:], lse[1:], q[1:], caches, table[1:], lens[1:], D ** -0.5)
+        before = [c.clone() for c in caches]
+        M.paged_moda_append(_rand(gen, BF, 2, 4, H, D), _rand(gen, BF, 2, 4, H, D), *caches, broken, torch.tensor([16, 50], dtype=torch.int32, device=DEV),
+                            torch.tensor([4, 0], dtype=torch.int32, device=DEV))
+        assert M.device_status() == (2 << 8 | 1)
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(caches, before))
+    room = table.shape[1] * page
+    full, ftable, _ = _pool(gen, BF, [room, room], 0, page, H, D)
+    for bad, seen in (([-5, room], [0, room]), ([room + 1, 3], [room, 3]), ([2 ** 31 - 1, -2 ** 31], [room, 0])):
+        n = torch.tensor(bad, dtype=torch.int32, device=DEV)
+        o, lse = M.paged_moda_decode(q, *full, ftable, n, moda_group_num=G, need_lse=True)
+        assert M.device_status() == (2 << 8 | 2)
+        _check_decode(o, lse, q, full, ftable, seen, D ** -0.5)
+        before = [c.clone() for c in full]
+        M.paged_moda_append(_rand(gen, BF, 2, 1, H, D), _rand(gen, BF, 2, 1, H, D), *full, ftable, n, torch.tensor([1, 0 if bad[1] == 3 else 1], dtype=torch.int32, device=DEV))
+        assert M.device_status() == (2 << 8 | 2)
+        assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(full, before))
+
+
+def test_offsets_past_32_bits(built_library):
+    """A pool of more than 2^32 bytes: the sequences' pages are its first and its last ones."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(13)
+    H, G, D, page = 8, 4, 128, 64
+    pages = (2 ** 31 + 2 ** 24) // (H * D * page)
+    caches = [torch.empty(pages, H, page, D, device=DEV, dtype=BF).transpose(1, 2) for _ in range(2)]
+    table = torch.tensor([[pages - 1, 0, pages - 2, pages - 3]], device=DEV, dtype=torch.int32)
+    for c in caches:
+        c[table[0].long()] = torch.randn(4, page, H, D, generator=gen, device=DEV).to(BF)
+    q, k, v = _rand(gen, BF, 1, G, H, D), _rand(gen, BF, 1, 1, H, D), _rand(gen, BF, 1, 1, H, D)
+    n = torch.tensor([200], dtype=torch.int32, device=DEV)
+    o, lse = M.paged_moda_decode(q, *caches, table, n, k, v, moda_group_num=G, need_lse=True)
+    _check_decode(o, lse, q, caches, table, [201], D ** -0.5)
+    assert torch.equal(caches[1][pages - 3, 200 - 192], v[0, 0])
+    M.paged_moda_append(k, v, *caches, table, torch.tensor([5], dtype=torch.int32, device=DEV))
+    assert torch.equal(caches[0][pages - 1, 5], k[0, 0])
+
+
+def test_refusals_on_the_gpu(built_library):
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(14)
+    caches, table, n = _pool(gen, BF, [5], 3, 8, 2, 64)
+    q, k = _rand(gen, BF, 1, 1, 2, 64), _rand(gen, BF, 1, 1, 2, 64)
+    with pytest.raises(RuntimeError, match="does not train"):
+        M.paged_moda_decode(q.clone().requires_grad_(), *caches, table, n)
+    with pytest.raises(RuntimeError, match="does not train"):
+        M.paged_moda_append(k.clone().requires_grad_(), k, *caches, table, n)
+    with torch.no_grad():
+        M.paged_moda_decode(q.clone().requires_grad_(), *caches, table, n)
+    with pytest.raises(AssertionError, match="dtype and device"):
+        M.paged_moda_decode(q.half(), *caches, table, n)
+    with pytest.raises(AssertionError, match="one device"):
+        M.paged_moda_decode(q, *caches, table.cpu(), n)
+    with pytest.raises(TypeError, match="bf16/fp16"):
+        M.paged_moda_append(k.float(), k.float(), caches[0].float(), caches[1].float(), table, n)
+    with pytest.raises(M.ModaLibraryError) as e:
+        M.paged_moda_append(k[:, :0], k[:, :0], *caches, table, n)
+    assert e.value.status == 2
+
+
+def test_captured_steps_follow_the_lengths(built_library):
+    """A decoding step is captured once and replayed while the sequences grow; two captured graphs and an eager call share nothing."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(15)
+    H, G, D, page, B = 2, 4, 128, 16, 3
+    lens = [900, 0, 33]
+    caches, table, n = _pool(gen, BF, lens, 12, page, H, D)
+    rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0])
+    q, k, v = _rand(gen, BF, B, G, H, D), _rand(gen, BF, B, 1, H, D), _rand(gen, BF, B, 1, H, D)
+
+    def step():
+        r = M.paged_moda_decode(q, *caches, table, n, k, v, rotary=rotary, moda_group_num=G, need_lse=True)
+        n.add_(1)
+        return r
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        graphs, outs = [], []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append(step())
+            graphs.append(graph)
+    torch.cuda.current_stream().wait_stream(side)
+    assert n.tolist() == [x + 1 for x in lens]
+    for i in range(5):
+        for x in (q, k, v):
+            x.copy_(_rand(gen, BF, *x.shape))
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        now = [x + 2 + i for x in lens]
+        assert n.tolist() == now
+        _check_decode(*outs[i % 2], q, caches, table, now, D ** -0.5, None, (rotary, n.long() - 1))
+    assert M.device_status() == 0
+
+
+def test_calls_on_two_streams_at_once(built_library):
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(16)
+    H, G, D, page = 4, 4, 128, 64
+    sets = []
+    for lens in ([6000, 10], [3000, 5000, 1]):
+        caches, table, n = _pool(gen, BF, lens, 0, page, H, D)
+        sets.append((lens, caches, table, n, _rand(gen, BF, len(lens), G, H, D)))
+    want = [M.paged_moda_decode(q, *caches, table, n, moda_group_num=G, need_lse=True) for _, caches, table, n, q in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(20):
+        for i, (_, caches, table, n, q) in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(M.paged_moda_decode(q, *caches, table, n, moda_group_num=G, need_lse=True))
+    torch.cuda.synchronize()
+    for w, gs in zip(want, got):
+        assert all(torch.equal(w[0], g[0]) and torch.equal(w[1], g[1]) for g in gs)
+
+
+@pytest.mark.parametrize("chunk_visible,G", [(False, 2), (False, 1), (True, 4)])
+def test_generating_with_a_stack_of_layers(built_library, chunk_visible, G):
+    """A prompt through the operators and its K/V into the caches, then tokens one by one: the attention of each layer at each new
+    position is what the operator over the whole sequence gives there."""
+    import moda_b200 as M
+    from oracle import moda_oracle as mo
+    gen = torch.Generator(device=DEV).manual_seed(17)
+    B, T0, T, H, D, N, page = 2, 37, 45, 2, 64, 4, 16
+    rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0])
+    C = 64 // G
+    layers = [tuple(_rand(gen, BF, B, T * r, H, D) for r in (G, 1, 1)) for _ in range(N)]
+    turned = [(*M.rotary_embedding(q, k, rotary, moda_group_num=G), v) for q, k, v in layers]
+    pages = [M.PagedKVCache(B * 3, page, H, D, BF, DEV) for _ in range(N)]
+    table = torch.arange(B * 3, device=DEV, dtype=torch.int32).view(B, 3)
+    n = torch.zeros(B, dtype=torch.int32, device=DEV)
+    for cache, (_, k, v) in zip(pages, layers):
+        cache.append(k[:, :T0], v[:, :T0], table, n, rotary=rotary)
+    n += T0
+    for t in range(T0, T):
+        first = t // C * C if chunk_visible else t                      # the positions whose depth rows the token sees
+        depth = M.DepthKVCache(B, t + 1 - first, N - 1, H, D, BF, DEV)
+        for i, (cache, (q, k, v)) in enumerate(zip(pages, layers)):
+            row = (q[:, t * G : (t + 1) * G], table, n, k[:, t : t + 1], v[:, t : t + 1])
+            if chunk_visible:
+                seen = torch.full((B,), t + 1 - first, dtype=torch.int32, device=DEV)
+                o, lse = cache.decode(*row, depth=depth, depth_positions=seen, moda_group_num=G, rotary=rotary, need_lse=True)
+                if i + 1 < N:
+                    depth.append(turned[i][1][:, first : t + 1], turned[i][2][:, first : t + 1])
+            else:
+                o, lse = cache.decode(*row, depth=depth, record=i + 1 < N, moda_group_num=G, rotary=rotary, need_lse=True)
+            assert depth.L == min(i + 1, N - 1)
+            qt, kt, vt = (x[:, : (t + 1) * r].float().cpu() for x, r in zip(turned[i], (G, 1, 1)))
+            kd, vd = (torch.stack([x[j][:, : t + 1] for x in turned[:i]], 2).flatten(1, 2).float().cpu() if i else None for j in (1, 2))
+            ref_o, ref_lse = mo.moda_attention_ref(qt, kt, vt, kd, vd, None, G, mo.MODE_CHUNK_VISIBLE if chunk_visible else mo.MODE_CAUSAL, C)
+            # The oracle takes q rounded to bf16, the step turns it without rounding: a score is off by 2^-9 of up to
+            # scale * sum |q k| (about 8 here, terms of either sign), and o by a few 2^-8 of values of about 1.
+            assert (o.float().cpu() - ref_o[:, -G:]).abs().max() <= 2e-2
+            assert (lse.cpu() - ref_lse[:, -G:]).abs().max() <= 2e-2
+        n += 1
+    for cache, (_, k, v) in zip(pages, turned):                         # and the caches hold every row
+        for b in range(B):
+            assert torch.equal(rows_of(cache.k, table[b], T), k[b]) and torch.equal(rows_of(cache.v, table[b], T), v[b])
+    assert M.device_status() == 0
