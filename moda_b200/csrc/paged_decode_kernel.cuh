@@ -36,17 +36,19 @@ constexpr int kMinTiles = 8;       // a CTA's range is not made shorter: two til
 struct DecodeParams {
   View q, o;                       // [B, G, H, D]
   Pages pages;
+  View k, v;                       // [B, 1, H, D]: the new tokens' own rows, which this call writes to the cache (pointers nullptr: none)
+  View k_copy, v_copy;             // [B, 1, H, D]: those rows as written once more (pointers nullptr: not)
   View kd, vd;                     // depth rows (b, layer, h); position p of P lies p * depth_sp further
   int64_t kd_sp, vd_sp;
   const int* depth_positions;      // [B]: positions seen, nullptr: all P
   int P, L;
   FastDiv by_L;
   float* lse;                      // [B, G, H]
-  rotary::Args rot;                // of the queries, at the last position of the sequence
+  rotary::Args rot;                // of the queries and the own keys, at the last position of the sequence
   int B, H, G;
-  int own_key;                     // 1: the sequences hold one row more than seq_lens says (written by this call)
   float scale_log2;
-  // scratch
+  int cluster;                     // 0: units are divided evenly over all CTAs; C: each unit over the C CTAs of a cluster
+  // scratch where units are divided over all CTAs
   int2* parts;                     // [CTA]: unit that is begun there and goes on in the next ones, and in how many it lies (0: none)
   float2* ml;                      // [CTA][2][kQ]: maximum and sum; part 0 goes on from the CTA before, part 1 begins here
   float* acc;                      // [CTA][2][kQ][D]
@@ -92,16 +94,21 @@ template <int D> __device__ __forceinline__ float4* part_at(float* parts, int wa
   return reinterpret_cast<float4*>(parts + (warp * kQ + row) * D) + (chunk ^ row);
 }
 
-struct Sequence { int len, keys, tiles; };          // rows in the cache, with the depth rows, 16-key tiles (at least one)
+struct Sequence { int held, len, keys, tiles; };     // rows in the cache, with the token's own, with the depth rows; 16-key tiles (at least one)
 __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
   Sequence s;
-  const int len = p.pages.seq_lens[b], room = p.pages.capacity();
-  s.len = len < 0 ? 0 : len >= room ? room : len + p.own_key;
+  const int room = p.pages.capacity();
+  s.held = min(max(p.pages.seq_lens[b], 0), room);
+  s.len = p.pages.seq_lens[b] >= 0 && s.held < room && p.k.ptr != nullptr ? s.held + 1 : s.held;
   const int P = p.depth_positions != nullptr ? min(max(p.depth_positions[b], 0), p.P) : p.P;
   const int64_t keys = (int64_t)s.len + (int64_t)P * p.L;
   s.keys = (int)(keys < 0x7ffffff0 ? keys : 0x7ffffff0);
   s.tiles = max((s.keys + kTile - 1) / kTile, 1);
   return s;
+}
+__device__ __forceinline__ void check_lengths(const DecodeParams& p, int b) {
+  const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : 0;
+  if (len < 0 || len > p.pages.capacity() - (p.k.ptr != nullptr) || seen < 0 || seen > p.P) wrong(kBadLength);
 }
 
 // A CTA's walk over its range of tiles: (sequence, unit of it, tiles [t0, t1) of the unit).
@@ -121,74 +128,118 @@ struct Walk {
   }
 };
 
-// The tiles of all units in a row, and this CTA's range of them.
-struct Range { int64_t total, begin, end; int n_cta; };
-template <int W> __device__ __forceinline__ int64_t block_sum(int64_t x, int64_t* s_part) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if (threadIdx.x % 32 == 0) s_part[threadIdx.x / 32] = x;
-  __syncthreads();
-  int64_t sum = 0;
-#pragma unroll
-  for (int i = 0; i < W; ++i) sum += s_part[i];
-  __syncthreads();
-  return sum;
+// The tiles of all units in a row, divided between n CTAs: CTA i has [begin(i), begin(i + 1)).
+struct Range {
+  int64_t total, each;               // each, and one more for some: the first `over` tiles are spread over the CTAs
+  uint32_t n, over;
+  __device__ __forceinline__ int64_t begin(uint32_t i) const { return each * i + (n != 0 ? over * i / n : 0u); }      // over, i <= n: the product fits
+};
+__device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {            // of numbers that nearly always fit 32 bits
+  return (a >> 32) == 0 ? (int64_t)((uint32_t)a / b) : a / b;
 }
+// This CTA's range and where it begins.  Every warp does it by itself: a lane takes four sequences of 128 at a time.
 __device__ __forceinline__ Walk locate(const DecodeParams& p, int units, Range& r) {
-  __shared__ int64_t s_part[kWarps];
-  __shared__ int s_b;
-  __shared__ int64_t s_first;
-  const int tid = threadIdx.x;
-  if (blockIdx.x == 0)
-    for (int b = tid; b < p.B; b += kThreads) {
-      const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : 0;
-      if (len < 0 || len > p.pages.capacity() - p.own_key || seen < 0 || seen > p.P) wrong(kBadLength);
+  const int lane = threadIdx.x & 31;
+  int64_t sum = 0;
+  int tiles[4];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = base + lane * 4 + k;
+      tiles[k] = b < p.B ? sequence(p, b).tiles : 0;
     }
-  const int tiles0 = tid < p.B ? sequence(p, tid).tiles : 0;
-  int64_t sum = tiles0;
-  for (int b = tid + kThreads; b < p.B; b += kThreads) sum += sequence(p, b).tiles;
-  r.total = block_sum<kWarps>(sum, s_part) * units;
-  r.n_cta = (int)min((int64_t)gridDim.x, (r.total + kMinTiles - 1) / kMinTiles);
-  const int i = blockIdx.x;
-  r.begin = r.end = 0;
+  };
+  for (int base = 0; base < p.B; base += 128) {
+    load(base);
+    sum += (int64_t)tiles[0] + tiles[1] + tiles[2] + tiles[3];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  r.total = sum * units;
+  r.n = (uint32_t)min((int64_t)gridDim.x, (r.total + kMinTiles - 1) / kMinTiles);
   Walk w{};
-  if (i >= r.n_cta) return w;
-  // total i / n without overflow: total below 2^47
-  r.begin = r.total / r.n_cta * i + r.total % r.n_cta * i / r.n_cta;
-  r.end = r.total / r.n_cta * (i + 1) + r.total % r.n_cta * (i + 1) / r.n_cta;
-  int64_t before = 0;
-  for (int base = 0;; base += kThreads) {                       // the sequence that holds tile `begin`
-    const int b = base + tid;
-    const int tiles = base == 0 ? tiles0 : b < p.B ? sequence(p, b).tiles : 0;
-    int64_t incl = (int64_t)tiles * units;
+  if (blockIdx.x >= r.n) return w;
+  r.each = quotient(r.total, r.n);
+  r.over = (uint32_t)(r.total - r.each * r.n);
+  const int64_t begin = r.begin(blockIdx.x);
+  w.left = r.begin(blockIdx.x + 1) - begin;
+  int64_t before = 0;                                           // tiles of the sequences before this lane's first one
+  for (int base = 0;; base += 128) {
+    if (p.B > 128) load(base);
+    const int64_t mine = ((int64_t)tiles[0] + tiles[1] + tiles[2] + tiles[3]) * units;
+    int64_t incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (tid % 32 >= o) incl += up;
+      if (lane >= o) incl += up;
     }
-    if (tid % 32 == 31) s_part[tid / 32] = incl;
-    __syncthreads();
-    int64_t start = before;
-    for (int j = 0; j < tid / 32; ++j) start += s_part[j];
-    const int64_t first = start + incl - (int64_t)tiles * units;
-    if (r.begin >= first && r.begin < start + incl) { s_b = b; s_first = first; }
-#pragma unroll
-    for (int j = 0; j < kWarps; ++j) before += s_part[j];
-    __syncthreads();
-    if (r.begin < before || base + kThreads >= p.B) break;      // uniform
+    const uint32_t here = __ballot_sync(0xffffffffu, begin < before + incl);
+    if (here != 0) {                                            // always at last: begin < total
+      const int from = __ffs(here) - 1;
+      int64_t off = begin - (before + incl - mine);
+      int k = 0;
+      for (; k < 3 && off >= (int64_t)tiles[k] * units; ++k) off -= (int64_t)tiles[k] * units;
+      off = __shfl_sync(0xffffffffu, off, from);
+      w.b = __shfl_sync(0xffffffffu, base + lane * 4 + k, from);
+      w.s = sequence(p, w.b);
+      w.unit = (int)quotient(off, (uint32_t)w.s.tiles);
+      w.t0 = (int)(off - (int64_t)w.unit * w.s.tiles);
+      w.cut();
+      return w;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  w.b = s_b;
+}
+// The same where a cluster of C CTAs has a unit: an even share of its tiles (none for some where there are few).
+__device__ __forceinline__ Walk locate_cluster(const DecodeParams& p, int units) {
+  Walk w{};
+  const int id = blockIdx.x / p.cluster, rank = blockIdx.x - id * p.cluster;
+  w.b = id / units;
+  w.unit = id - w.b * units;
   w.s = sequence(p, w.b);
-  const int64_t off = r.begin - s_first;
-  w.unit = (int)(off / w.s.tiles);
-  w.t0 = (int)(off % w.s.tiles);
-  w.left = r.end - r.begin;
-  w.cut();
+  w.t0 = (int)((int64_t)w.s.tiles * rank / p.cluster);
+  w.t1 = (int)((int64_t)w.s.tiles * (rank + 1) / p.cluster);
+  w.left = w.t1 - w.t0;
   return w;
 }
 
+// The new token's own row of head h: turned, written to its place in the cache (page, slot) and to the copies, and the key to its
+// place in the tile in shared memory (row n of the tile at `tile_k`; the value is copied there like any other).  Rare (once a unit),
+// and kept out of line so that the loop's registers are not laid out for it.
+template <typename T, int D>
+__device__ __noinline__ void own_row(const DecodeParams& p, int b, int h, int page, int slot, int position, bool write, uint32_t tile_k, int n) {
+  constexpr int C = D / 16;
+  const int lane = threadIdx.x & 31, c = lane % C;
+  float2 cs[8];
+  if (p.rot.inv_freq != nullptr) rotary::item_cos_sin<C>(p.rot, lane, position, cs);
+  if (lane >= 2 * C) return;
+  const bool of_v = lane >= C;
+  const View& in = of_v ? p.v : p.k;
+  int c0, c1;
+  const bool turns = rotary::item_chunks(p.rot, c, c0, c1) && p.rot.inv_freq != nullptr && !of_v;
+  uint4 x = *rotary::chunk_at(in, in.off(b, 0, h), c0), y = *rotary::chunk_at(in, in.off(b, 0, h), c1);
+  if (turns) rotary::turn<T>(x, y, cs, p.rot.interleaved != 0);
+  if (write) {
+    const View &to = of_v ? p.pages.v : p.pages.k, &copy = of_v ? p.v_copy : p.k_copy;
+    *rotary::chunk_at(to, to.off(page, slot, h), c0) = x;
+    *rotary::chunk_at(to, to.off(page, slot, h), c1) = y;
+    if (copy.ptr != nullptr) {
+      *rotary::chunk_at(copy, copy.off(b, 0, h), c0) = x;
+      *rotary::chunk_at(copy, copy.off(b, 0, h), c1) = y;
+    }
+  }
+  if (!of_v) {
+    const uint32_t row = tile_k + n * D * 2;
+    auto put = [&](int chunk, const uint4& z) {
+      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(row + ((chunk ^ k_swizzle(n)) << 4)), "r"(z.x), "r"(z.y), "r"(z.z), "r"(z.w) : "memory");
+    };
+    put(c0, x);
+    put(c1, y);
+  }
+}
+
 // Copies the tiles of one warp, ahead of their use.
-template <int D> struct Loader {
+template <typename T, int D> struct Loader {
   Walk w;
   int tile;                          // this warp's next one, of w
   int page;                          // of this lane's key in it, fetched ahead
@@ -233,7 +284,7 @@ template <int D> struct Loader {
       const uint32_t slot = ring + stage * stage_bytes<D>();
       const int which = (int)p.pages.by_page.div((uint32_t)first), row0 = first - which * p.pages.page_size;
       const int page0 = __shfl_sync(0xffffffffu, page, 0);
-      if (first + kTile <= w.s.len && row0 + kTile <= p.pages.page_size && page0 >= 0 && page0 < p.pages.num_pages) {
+      if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page0 >= 0 && page0 < p.pages.num_pages) {
         // sixteen rows of one page
         if (lane == 0) masks[stage] = 0xffffu;
         const unsigned char* k = reinterpret_cast<const unsigned char*>(rotary::chunk_at(p.pages.k, p.pages.k.off(page0, row0 + r, h), c));
@@ -245,31 +296,37 @@ template <int D> struct Loader {
       } else {
         // each row by itself: lane l finds the K row (l < 16) or the V row of key l % 16
         const int key = first + (lane & 15);
-        const bool of_v = lane >= 16;
+        const bool of_v = lane >= 16, own = key >= w.s.held && key < w.s.len;
         const View &cache = of_v ? p.pages.v : p.pages.k, &depth = of_v ? p.vd : p.kd;
         bool valid = key < w.s.keys;
         const unsigned char* row = static_cast<const unsigned char*>(cache.ptr);
+        int slot_of = 0;
         if (key < w.s.len) {
           if (page >= 0 && page < p.pages.num_pages) {
-            const int slot_of = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
-            row += 2 * cache.off(page, slot_of, h);
+            slot_of = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
+            row = own ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h) : row + 2 * cache.off(page, slot_of, h);
           } else {
             valid = false;
             wrong(kBadPage);
           }
         } else if (valid) {
-          const int c = key - w.s.len, pos = (int)p.by_L.div((uint32_t)c), layer = c - pos * p.L;
+          const int d = key - w.s.len, pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
           row = static_cast<const unsigned char*>(depth.ptr) + 2 * (depth.off(w.b, layer, h) + pos * (of_v ? p.vd_sp : p.kd_sp));
         }
-        const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu;
+        const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own && valid) & 0xffffu;
         if (lane == 0) masks[stage] = there;
         const unsigned long long at = reinterpret_cast<unsigned long long>(row);
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
           const int n = i * kRows + r;
           const bool ok = (there >> n) & 1u;
-          copy_k(slot, i, reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, at, n) + c * 16), ok);
-          copy_v(slot, i, reinterpret_cast<const void*>(__shfl_sync(0xffffffffu, at, 16 + n) + c * 16), ok);
+          const unsigned long long k = __shfl_sync(0xffffffffu, at, n) + c * 16, v = __shfl_sync(0xffffffffu, at, 16 + n) + c * 16;
+          if (!((its_own >> n) & 1u)) copy_k(slot, i, reinterpret_cast<const void*>(k), ok);
+          copy_v(slot, i, reinterpret_cast<const void*>(v), ok);
+        }
+        if (its_own != 0) {
+          const int n = __ffs(its_own) - 1;
+          own_row<T, D>(p, w.b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), w.s.held, w.unit == h * query_blocks, slot, n);
         }
       }
       tile += kWarps;
@@ -280,12 +337,47 @@ template <int D> struct Loader {
   }
 };
 
+// Joins the parts that the CTAs of a cluster hold in their shared memory: rows of D at `acc`, maxima and sums at `ml`.  Each CTA
+// takes every C-th group of four elements.
+template <typename T, int D>
+__device__ __forceinline__ void join_cluster(const DecodeParams& p, const Walk& w, int h, int q0, uint32_t acc, uint32_t ml) {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+  uint32_t rank;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  for (int i = threadIdx.x * p.cluster + rank; i < kQ * D / 4; i += kThreads * p.cluster) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    if (q0 + r >= p.G) break;
+    float top = -INFINITY, sum = 0.f;
+    float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = 0; c < p.cluster; ++c) {
+      uint32_t at;
+      float2 x;
+      float4 y;
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ml + r * 8), "r"(c));
+      asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(acc + (r * D + d) * 4), "r"(c));
+      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(at) : "memory");
+      const float now = fmaxf(top, x.x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(x.x - base);
+      sum = sum * a + x.y * b;
+      out = make_float4(out.x * a + y.x * b, out.y * a + y.y * b, out.z * a + y.z * b, out.w * a + y.w * b);
+      top = now;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint2* to = reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d));
+    *to = make_uint2(Pack<T>::pack(out.x * inv, out.y * inv), Pack<T>::pack(out.z * inv, out.w * inv));
+    if (d == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
+  }
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");      // nobody leaves while it is read
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint32_t s_masks[kWarps][stages<D>()];
   __shared__ float2 s_ml[kWarps][kQ];
   __shared__ float2 s_cs[D / 2];
+  __shared__ float2 s_part_ml[kQ];
   constexpr int kStages = stages<D>();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
   const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
@@ -293,13 +385,21 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   float* s_acc = reinterpret_cast<float*>(smem + (size_t)kWarps * kStages * stage_bytes<D>());
 
   grid_started();
-  Range range;
-  Walk w = locate(p, units, range);
-  if (range.begin == range.end) {
-    if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
-    return;
+  Range range{};
+  Walk w;
+  if (p.cluster != 0) {
+    w = locate_cluster(p, units);
+    if (w.unit == 0 && w.t0 == 0 && tid == 0) check_lengths(p, w.b);
+  } else {
+    w = locate(p, units, range);
+    if (w.left == 0) {
+      if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
+      return;
+    }
+    if (blockIdx.x == 0)
+      for (int b = tid; b < p.B; b += kThreads) check_lengths(p, b);
   }
-  Loader<D> loader;
+  Loader<T, D> loader;
   loader.start(p, units, warp, w, ring);
 #pragma unroll
   for (int s = 0; s < kStages; ++s) loader.issue(p, units, query_blocks, warp, s_masks[warp]);
@@ -308,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   const uint32_t k_even = g * D * 2 + (t ^ k_swizzle(g)) * 16, k_odd = g * D * 2 + ((4 + t) ^ k_swizzle(g)) * 16;
   const uint32_t v_even = kTile * D * 2 + 2 * t * D * 2 + (g ^ (2 * t)) * 16, v_odd = kTile * D * 2 + (2 * t + 1) * D * 2 + (g ^ (2 * t + 1)) * 16;
   int stage = 0, turned_b = -1;
-  int64_t at = range.begin;                  // the walk's place in the row of all tiles
+  int64_t at = range.begin(blockIdx.x);      // the walk's place in the row of all tiles
   int2 part = make_int2(0, 0);
   bool going = true;
   while (going) {
@@ -316,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     const bool row_there = q0 + g < p.G;
     if (p.rot.inv_freq != nullptr && turned_b != w.b) {
       __syncthreads();
-      for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], (long long)w.s.len - 1);
+      for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
       __syncthreads();
       turned_b = w.b;
     }
@@ -435,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     }
     __syncthreads();
     const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
+    const bool whole = p.cluster != 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
     constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
     const int r = tid / 16, d0 = (tid % 16) * kEach;
     if (q0 + r < p.G) {
@@ -456,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           out[e + 3] = fmaf(x.w, weight, out[e + 3]);
         }
       }
-      if (from_start && to_end) {
+      if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         uint32_t packed[kEach / 2];
 #pragma unroll
@@ -465,20 +566,23 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
         if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
-      } else {
-        const int64_t at_row = ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
+      } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
+        const int64_t at_row = p.cluster != 0 ? r : ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
+        float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) p.acc[at_row * D + d0 + e] = out[e];
-        if (d0 == 0) p.ml[at_row] = make_float2(top, sum);
+        for (int e = 0; e < kEach; ++e) to[e] = out[e];
+        if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
       }
+    }
+    if (p.cluster != 0) {
+      if (!whole) join_cluster<T, D>(p, w, h, q0, smem_u32(smem), smem_u32(s_part_ml));
+      return;
     }
     if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
       const int64_t last = at + w.s.tiles - 1;
-      int64_t n = (last - (range.end - 1) + range.total / range.n_cta - 1) / max(range.total / range.n_cta, (int64_t)1);
-      // ranges differ by one tile at most: correct the estimate
-      auto begin_of = [&](int64_t i) { return range.total / range.n_cta * i + range.total % range.n_cta * i / range.n_cta; };
-      while (n > 1 && begin_of(blockIdx.x + n) > last) --n;
-      while (begin_of(blockIdx.x + n + 1) <= last) ++n;
+      uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
+      while (range.begin(blockIdx.x + n) > last) --n;
+      while (range.begin(blockIdx.x + n + 1) <= last) ++n;
       part = make_int2(w.b * units + w.unit, (int)n + 1);
     }
     at += w.t1 - w.t0;
@@ -491,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float s_acc[kWarps][D];
-  __shared__ float s_sum[kWarps];
+  __shared__ float2 s_ml[kWarps];
   grid_before();
   const int2 part = p.parts[blockIdx.x];
   const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
@@ -499,34 +603,39 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   if (part.y < 2 || row >= p.G) return;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   auto place = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
-  float top = -INFINITY;
-  for (int i = lane; i < part.y; i += 32) top = fmaxf(top, p.ml[place(i)].x);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float base = top == -INFINITY ? 0.f : top;
   constexpr int kEach = D / 32;
-  float sum = 0.f, out[kEach] = {};
+  float top = -INFINITY, sum = 0.f, out[kEach] = {};
 #pragma unroll 4
   for (int i = warp; i < part.y; i += kWarps) {
     const float2 ml = p.ml[place(i)];
-    const float weight = fast_exp2(ml.x - base);
-    sum = fmaf(ml.y, weight, sum);
-    const float* x = p.acc + place(i) * D + lane * kEach;
+    float x[kEach];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) out[e] = fmaf(x[e], weight, out[e]);
+    for (int e = 0; e < kEach; ++e) x[e] = p.acc[place(i) * D + lane * kEach + e];
+    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(ml.x - base);
+    sum = sum * a + ml.y * b;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) out[e] = out[e] * a + x[e] * b;
+    top = now;
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) s_acc[warp][lane * kEach + e] = out[e];
-  if (lane == 0) s_sum[warp] = sum;
+  if (lane == 0) s_ml[warp] = make_float2(top, sum);
   __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float weight[kWarps];
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) sum += s_sum[i];
+  for (int i = 0; i < kWarps; ++i) {
+    weight[i] = fast_exp2(s_ml[i].x - base);
+    sum = fmaf(s_ml[i].y, weight[i], sum);
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   for (int d = threadIdx.x; d < D / 2; d += kThreads) {
     float x = 0.f, y = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) { x += s_acc[i][2 * d]; y += s_acc[i][2 * d + 1]; }
+    for (int i = 0; i < kWarps; ++i) { x = fmaf(s_acc[i][2 * d], weight[i], x); y = fmaf(s_acc[i][2 * d + 1], weight[i], y); }
     reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * p.o.off(b, row, h))[d] = Pack<T>::pack(x * inv, y * inv);
   }
   if (threadIdx.x == 0) p.lse[((int64_t)b * p.G + row) * p.H + h] = top + log2f(sum);

@@ -199,7 +199,6 @@ struct AppendParams {
   Pages pages;
   const int* lengths;        // [B], nullptr: T tokens each
   rotary::Args rot;          // of the keys
-  View k_copy, v_copy;       // [B, T, H, D]: the rows as written once more (pointers nullptr: not)
   int B, T, H;
   int per_warp;              // of a token's 2 H vectors
   FastDiv by_t;
@@ -251,12 +250,6 @@ __global__ void __launch_bounds__(rotary::kThreads) append_kernel(const __grid_c
         const int64_t off = to.off(page, slot, v < p.H ? v : v - p.H);
         *chunk_at(to, off, c0) = x[i];
         *chunk_at(to, off, c1) = y[i];
-        if (p.k_copy.ptr != nullptr) {
-          const View& copy = v < p.H ? p.k_copy : p.v_copy;
-          const int64_t at = copy.off(b, t, v < p.H ? v : v - p.H);
-          *chunk_at(copy, at, c0) = x[i];
-          *chunk_at(copy, at, c1) = y[i];
-        }
       }
     }
   }

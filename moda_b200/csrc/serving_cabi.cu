@@ -70,9 +70,8 @@ template <typename T, int D> void launch_append(const paged::AppendParams& p, di
 }
 
 int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v, const paged::Pages& pages, const int32_t* lengths,
-           const rotary::Args& rot, const moda_tensor4* k_copy, const moda_tensor4* v_copy, int n_sm, cudaStream_t st) {
+           const rotary::Args& rot, int n_sm, cudaStream_t st) {
   paged::AppendParams p{};
-  p.k_copy = to_view(k_copy); p.v_copy = to_view(v_copy);
   p.k = to_view(k); p.v = to_view(v); p.pages = pages; p.lengths = lengths; p.rot = rot;
   p.B = pr->B; p.T = pr->T_kv; p.H = pr->H; p.by_t = rotary::FastDiv((uint32_t)pr->T_kv);
   const dim3 grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm, &p.per_warp);
@@ -87,8 +86,18 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
   return MODA_OK;
 }
 
-int decode_ctas(int n_sm) { return 2 * n_sm; }
-// Scratch: which units are shared, their parts' maxima and sums, their parts.
+// How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
+// the width of its table.
+struct Division { int ctas, cluster; };
+Division divide(const moda_problem* pr, int64_t most_keys, int n_sm) {
+  const int64_t heads = (int64_t)pr->H * ((pr->G + paged::kQ - 1) / paged::kQ), units = pr->B * heads;
+  const int64_t tiles = std::max<int64_t>(1, (most_keys + paged::kTile - 1) / paged::kTile), slots = 2 * n_sm;
+  int cluster = 1;
+  while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
+  if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
+  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, units * tiles / paged::kMinTiles)), 0};
+}
+// Scratch of an evenly divided call: which units are shared, their parts' maxima and sums, their parts.
 size_t parts_bytes(int n) { return ((size_t)n * sizeof(int2) + 255) & ~(size_t)255; }
 size_t ml_bytes(int n) { return (size_t)n * 2 * paged::kQ * sizeof(float2); }
 size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * 2 * paged::kQ * D * sizeof(float); }
@@ -97,22 +106,32 @@ template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta,
   auto kern = paged::decode_kernel<T, D>;
   constexpr size_t smem = paged::smem_bytes<D>();
   if (int rc = opt_in_smem(kern, smem)) return rc;
-  {
-    prof::Scope ps(prof::kPagedDecode, st);
-    kern<<<n_cta, paged::kThreads, smem, st>>>(p);
-  }
-  MODA_CUDA(cudaGetLastError());
-  g_last_launches += 1;
   cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(n_cta, std::min(p.G, paged::kQ));
+  cfg.gridDim = dim3(n_cta);
   cfg.blockDim = dim3(paged::kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = std::max(p.cluster, 1);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  if (p.cluster > 8) MODA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaError_t e;
+  {
+    prof::Scope ps(prof::kPagedDecode, st);
+    e = cudaLaunchKernelEx(&cfg, kern, p);
+  }
+  MODA_CUDA(e);
+  g_last_launches += 1;
+  if (p.cluster != 0) return MODA_OK;
+  cfg.gridDim = dim3(n_cta, std::min(p.G, paged::kQ));
+  cfg.dynamicSmemBytes = 0;
+  cfg.numAttrs = 1;
+  attr = cudaLaunchAttribute{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   {
     prof::Scope ps(prof::kPagedJoin, st);
     e = cudaLaunchKernelEx(&cfg, paged::join_kernel<T, D>, p);
@@ -193,7 +212,7 @@ int moda_b200_paged_append(const moda_problem* prob, const moda_tensor4* k, cons
   g_last_launches = 0;
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  return append(prob, k, v, pages, lengths, turn, nullptr, nullptr, n_sm, reinterpret_cast<cudaStream_t>(stream));
+  return append(prob, k, v, pages, lengths, turn, n_sm, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, size_t* bytes) {
@@ -201,7 +220,7 @@ int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, size_t* byt
   if (int rc = check_sizes(prob)) return rc;
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  *bytes = decode_scratch(decode_ctas(n_sm), prob->D);
+  *bytes = decode_scratch(2 * n_sm, prob->D);
   return MODA_OK;
 }
 
@@ -245,20 +264,22 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   if (!guard.ok) return cuda_fail(guard.err);
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  const int n_cta = decode_ctas(n_sm);
-  if (workspace == nullptr || workspace_bytes < decode_scratch(n_cta, prob->D)) return MODA_ERR_WORKSPACE;
+  const Division div = divide(prob, (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L, n_sm);
+  const int n_cta = div.ctas;
+  p.cluster = div.cluster;
+  if (workspace == nullptr || workspace_bytes < decode_scratch(2 * n_sm, prob->D)) return MODA_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.q = to_view(q); p.o = to_view(o); p.lse = lse;
-  p.B = prob->B; p.H = prob->H; p.G = prob->G; p.own_key = own_key;
+  p.B = prob->B; p.H = prob->H; p.G = prob->G;
+  p.k = to_view(own_key ? k : nullptr); p.v = to_view(own_key ? v : nullptr);
+  p.k_copy = to_view(own_key ? k_copy : nullptr); p.v_copy = to_view(own_key ? v_copy : nullptr);
   p.scale_log2 = prob->scale * 1.4426950408889634f;
   p.parts = reinterpret_cast<int2*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + parts_bytes(n_cta));
   p.acc = reinterpret_cast<float*>(ws + parts_bytes(n_cta) + ml_bytes(n_cta));
   g_last_launches = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (own_key)
-    if (int rc = append(prob, k, v, p.pages, nullptr, p.rot, k_copy, v_copy, n_sm, st)) return rc;
   const bool bf = prob->dtype == MODA_BF16;
   if (prob->D == 128) return bf ? decode<__nv_bfloat16, 128>(p, n_cta, st) : decode<__half, 128>(p, n_cta, st);
   return bf ? decode<__nv_bfloat16, 64>(p, n_cta, st) : decode<__half, 64>(p, n_cta, st);
