@@ -11,14 +11,14 @@
 //    range, which may end one unit, hold several and begin another.  A unit that lies in one CTA's range is
 //    written at once, the others' parts are joined by a second, dependent launch.
 //  - A warp takes every fourth tile of the CTA's range and copies it, asynchronously, into slots of shared memory of its
-//    own, kStages tiles ahead and across the ends of units: warps do not wait for one another.  An instruction copies
+//    own, kStages - 1 tiles ahead and across the ends of units: warps do not wait for one another.  An instruction copies
 //    whole rows (512 bytes in one piece where a page holds its heads one after another).  Measured on 1 GB: 7.0 TB/s, against
 //    5.0 where a lane copies the chunks that it will multiply, eight rows and 64 bytes of each an instruction.
 //  - The products are m16n8k16 matrix instructions.  At 16 keys a tile and 8 query rows their rate is far from a
 //    limit (32 instructions a tile of 8 KB at D = 128), so that tcgen05 tiles of 128 keys, which need barriers, TMEM and
-//    16 times the padding, would buy nothing.  The order of the head's elements within a product and the order of V's
-//    columns are free, and are chosen so that each operand is a 16-byte chunk of a row: K: lane (g, t) = (lane / 4,
-//    lane % 4) holds elements 32 j + 8 t .. + 7 of key g; V: elements 64 j + 8 g .. + 7 of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+//    16 times the padding, would buy nothing.  The order of the head's elements within a score is free, and is chosen so
+//    that a lane's operands are 16-byte chunks of a row: lane (g, t) = (lane / 4, lane % 4) holds elements 32 j + 8 t .. + 7 of
+//    key g.  V is read transposed by the matrix loads.
 //  - Eight query rows leave the lower half of the 16-row operand free.  It holds what rounding the upper half to 16
 //    bits has left over: the rotated query's remainder (the query is turned here, in 32 bits, without rounding), and that of
 //    the probabilities.  So neither is rounded to fewer than 16 significant bits, at no cost.
@@ -83,9 +83,15 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
 
 // A tile in shared memory: 16 rows of K, 16 of V.  Chunk c (16 bytes) of row r is at place c ^ k_swizzle(r) of its row, or c ^ (r & 7):
 // the eight lanes that an access takes together then meet all banks, for the copies (chunks of one row) as for the reads
-// (K: chunks 4 j + t of two neighbouring rows g; V: chunks g of rows 2 t + b).
+// (K: chunks 4 j + t of two neighbouring rows g; V: one chunk of eight rows).
+// Four 8 x 8 matrices of 16-bit values, transposed: lane l gives the address of row l % 8 of matrix l / 8, and gets of each matrix the
+// elements of column l / 4 in rows 2 (l % 4) and the next.
+__device__ __forceinline__ void load_transposed(uint32_t (&x)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
+
 template <int D> __host__ __device__ constexpr int stage_bytes() { return kTile * D * 2 * 2; }
-__device__ __forceinline__ int k_swizzle(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
+__host__ __device__ constexpr int k_swizzle(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
 template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }      // 24 KB a warp
 // The copies' slots and the warps' parts of a unit.  With what the kernel declares statically, two CTAs just fit an SM.
 template <int D> constexpr size_t smem_bytes() { return (size_t)kWarps * stages<D>() * stage_bytes<D>() + (size_t)kWarps * kQ * D * 4; }
@@ -204,10 +210,9 @@ __device__ __forceinline__ Walk locate_cluster(const DecodeParams& p, int units)
 }
 
 // The new token's own row of head h: turned, written to its place in the cache (page, slot) and to the copies, and the key to its
-// place in the tile in shared memory (row n of the tile at `tile_k`; the value is copied there like any other).  Rare (once a unit),
-// and kept out of line so that the loop's registers are not laid out for it.
+// place in the tile in shared memory (row n of the tile at `tile_k`; the value is copied there like any other).
 template <typename T, int D>
-__device__ __noinline__ void own_row(const DecodeParams& p, int b, int h, int page, int slot, int position, bool write, uint32_t tile_k, int n) {
+__device__ __forceinline__ void own_row(const DecodeParams& p, int b, int h, int page, int slot, int position, bool write, uint32_t tile_k, int n) {
   constexpr int C = D / 16;
   const int lane = threadIdx.x & 31, c = lane % C;
   float2 cs[8];
@@ -238,6 +243,58 @@ __device__ __noinline__ void own_row(const DecodeParams& p, int b, int h, int pa
   }
 }
 
+// Copies a tile's rows one by one: the ones that a page's end divides, the last ones of a sequence, its own row and the depth rows.
+// Lane l finds the K row (l < 16) or the V row of key first + l % 16, whose page is `page`.  Out of line: the loop's code stays small, and its
+// registers are not laid out for this.
+template <typename T, int D>
+__device__ __noinline__ void mixed_tile(const DecodeParams& p, int b, const Sequence s, int h, bool write, int first, int page, uint32_t slot, uint32_t* mask) {
+  constexpr int kChunks = D / 8, kRows = 32 / kChunks, kCopies = kTile / kRows;
+  const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
+  const int key = first + (lane & 15);
+  const bool of_v = lane >= 16, own = key >= s.held && key < s.len;
+  const View &cache = of_v ? p.pages.v : p.pages.k, &depth = of_v ? p.vd : p.kd;
+  bool valid = key < s.keys;
+  const unsigned char* row = static_cast<const unsigned char*>(cache.ptr);
+  int slot_of = 0;
+  if (key < s.len) {
+    if (page >= 0 && page < p.pages.num_pages) {
+      slot_of = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
+      row = own ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(b, 0, h) : row + 2 * cache.off(page, slot_of, h);
+    } else {
+      valid = false;
+      wrong(kBadPage);
+    }
+  } else if (valid) {
+    const int d = key - s.len, pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
+    row = static_cast<const unsigned char*>(depth.ptr) + 2 * (depth.off(b, layer, h) + pos * (of_v ? p.vd_sp : p.kd_sp));
+  }
+  const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own && valid) & 0xffffu;
+  if (lane == 0) *mask = there;
+  const unsigned long long at = reinterpret_cast<unsigned long long>(row);
+#pragma unroll 2
+  for (int i = 0; i < kCopies; ++i) {
+    const int n = i * kRows + r;
+    const bool ok = (there >> n) & 1u;
+    const unsigned long long k = __shfl_sync(0xffffffffu, at, n) + c * 16, v = __shfl_sync(0xffffffffu, at, 16 + n) + c * 16;
+    if (!((its_own >> n) & 1u)) copy16(slot + n * D * 2 + ((c ^ k_swizzle(n)) << 4), reinterpret_cast<const void*>(k), ok);
+    copy16(slot + (kTile + n) * D * 2 + ((c ^ (n & 7)) << 4), reinterpret_cast<const void*>(v), ok);
+  }
+  if (its_own != 0) {
+    const int n = __ffs(its_own) - 1;
+    own_row<T, D>(p, b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), s.held, write, slot, n);
+  }
+}
+
+// A tile's K (or V) rows, each `stride` elements behind the one before.  `from`: this lane's chunk of the first copy's row, which goes to
+// `to`.  The rows of copy i swizzle as those of the first do, but for bits that are known of i.
+template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to, const void* from, int64_t stride) {
+  constexpr int kRows = 32 / (D / 8), kCopies = kTile / kRows;
+  const unsigned char* at = static_cast<const unsigned char*>(from);
+#pragma unroll
+  for (int i = 0; i < kCopies; ++i, at += kRows * 2 * stride)
+    copy16((to ^ ((kV ? i * kRows & 7 : k_swizzle(i * kRows & 7)) << 4)) + i * kRows * D * 2, at, true);
+}
+
 // Copies the tiles of one warp, ahead of their use.
 template <typename T, int D> struct Loader {
   Walk w;
@@ -248,7 +305,7 @@ template <typename T, int D> struct Loader {
   int stage;
   uint32_t to_k, to_v;               // where this lane's chunk of the first copy goes in a stage; the others' follow by the swizzle
 
-  static constexpr int kChunks = D / 8, kRows = 32 / kChunks, kCopies = kTile / kRows;      // of a row; rows of a copy; copies of a tile's K
+  static constexpr int kChunks = D / 8;
 
   __device__ __forceinline__ void settle(const DecodeParams& p, int units, int warp) {      // at a tile of this warp, or at the end
     while (more && tile >= w.t1) {
@@ -269,13 +326,6 @@ template <typename T, int D> struct Loader {
     to_v = kTile * D * 2 + r * D * 2 + (c ^ r) * 16;
     settle(p, units, warp);
   }
-  // Row kRows i + r swizzles as row r does, but for bits that are known of i.
-  __device__ __forceinline__ void copy_k(uint32_t slot, int i, const void* from, bool ok) const {
-    copy16((slot + to_k + i * kRows * D * 2) ^ (k_swizzle((i * kRows) & 7) << 4), from, ok);
-  }
-  __device__ __forceinline__ void copy_v(uint32_t slot, int i, const void* from, bool ok) const {
-    copy16((slot + to_v + i * kRows * D * 2) ^ (((i * kRows) & 7) << 4), from, ok);
-  }
   // Issues the copies of one tile (none at the end); `mask` in shared memory gets a bit for each key that is there.
   __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, int warp, uint32_t* masks) {
     if (more) {
@@ -287,47 +337,10 @@ template <typename T, int D> struct Loader {
       if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page0 >= 0 && page0 < p.pages.num_pages) {
         // sixteen rows of one page
         if (lane == 0) masks[stage] = 0xffffu;
-        const unsigned char* k = reinterpret_cast<const unsigned char*>(rotary::chunk_at(p.pages.k, p.pages.k.off(page0, row0 + r, h), c));
-        const unsigned char* v = reinterpret_cast<const unsigned char*>(rotary::chunk_at(p.pages.v, p.pages.v.off(page0, row0 + r, h), c));
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) copy_k(slot, i, k + i * (kRows * 2 * p.pages.k.st), true);
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) copy_v(slot, i, v + i * (kRows * 2 * p.pages.v.st), true);
+        copy_rows<D, false>(slot + to_k, rotary::chunk_at(p.pages.k, p.pages.k.off(page0, row0 + r, h), c), p.pages.k.st);
+        copy_rows<D, true>(slot + to_v, rotary::chunk_at(p.pages.v, p.pages.v.off(page0, row0 + r, h), c), p.pages.v.st);
       } else {
-        // each row by itself: lane l finds the K row (l < 16) or the V row of key l % 16
-        const int key = first + (lane & 15);
-        const bool of_v = lane >= 16, own = key >= w.s.held && key < w.s.len;
-        const View &cache = of_v ? p.pages.v : p.pages.k, &depth = of_v ? p.vd : p.kd;
-        bool valid = key < w.s.keys;
-        const unsigned char* row = static_cast<const unsigned char*>(cache.ptr);
-        int slot_of = 0;
-        if (key < w.s.len) {
-          if (page >= 0 && page < p.pages.num_pages) {
-            slot_of = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
-            row = own ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h) : row + 2 * cache.off(page, slot_of, h);
-          } else {
-            valid = false;
-            wrong(kBadPage);
-          }
-        } else if (valid) {
-          const int d = key - w.s.len, pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
-          row = static_cast<const unsigned char*>(depth.ptr) + 2 * (depth.off(w.b, layer, h) + pos * (of_v ? p.vd_sp : p.kd_sp));
-        }
-        const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own && valid) & 0xffffu;
-        if (lane == 0) masks[stage] = there;
-        const unsigned long long at = reinterpret_cast<unsigned long long>(row);
-#pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
-          const int n = i * kRows + r;
-          const bool ok = (there >> n) & 1u;
-          const unsigned long long k = __shfl_sync(0xffffffffu, at, n) + c * 16, v = __shfl_sync(0xffffffffu, at, 16 + n) + c * 16;
-          if (!((its_own >> n) & 1u)) copy_k(slot, i, reinterpret_cast<const void*>(k), ok);
-          copy_v(slot, i, reinterpret_cast<const void*>(v), ok);
-        }
-        if (its_own != 0) {
-          const int n = __ffs(its_own) - 1;
-          own_row<T, D>(p, w.b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), w.s.held, w.unit == h * query_blocks, slot, n);
-        }
+        mixed_tile<T, D>(p, w.b, w.s, h, w.unit == h * query_blocks, first, page, slot, masks + stage);
       }
       tile += kWarps;
       settle(p, units, warp);
@@ -401,12 +414,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   }
   Loader<T, D> loader;
   loader.start(p, units, warp, w, ring);
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) loader.issue(p, units, query_blocks, warp, s_masks[warp]);
+#pragma unroll 1
+  for (int s = 0; s < kStages - 1; ++s) loader.issue(p, units, query_blocks, warp, s_masks[warp]);
 
-  // places of this lane's chunks in a stage: K of row g (even and odd j), V of rows 2 t and 2 t + 1
+  // places of this lane's chunks in a stage: K of row g (even and odd j), V of row lane % 16, chunk lane / 16
   const uint32_t k_even = g * D * 2 + (t ^ k_swizzle(g)) * 16, k_odd = g * D * 2 + ((4 + t) ^ k_swizzle(g)) * 16;
-  const uint32_t v_even = kTile * D * 2 + 2 * t * D * 2 + (g ^ (2 * t)) * 16, v_odd = kTile * D * 2 + (2 * t + 1) * D * 2 + (g ^ (2 * t + 1)) * 16;
+  const uint32_t v_place = (kTile + lane % 16) * D * 2 + ((lane >> 4) ^ (lane & 7)) * 16;
   int stage = 0, turned_b = -1;
   int64_t at = range.begin(blockIdx.x);      // the walk's place in the row of all tiles
   int2 part = make_int2(0, 0);
@@ -463,26 +476,32 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 
     for (int tile = w.t0 + warp; tile < w.t1; tile += kWarps) {
-      copies_wait<kStages - 1>();
-      __syncwarp();                          // the other lanes' copies, and the mask
+      copies_wait<kStages - 2>();
+      __syncwarp();                          // the other lanes' copies, and the mask; and all lanes have read the tile before
       const uint32_t mask = s_masks[warp][stage];
       const uint32_t slot = ring + stage * stage_bytes<D>();
-      float s[2][4];
+      float s[2][4], s2[2][4];               // two sums each: the products of one wait for one another
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
-        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const uint4 k = lds128(slot + (j & 1 ? k_odd : k_even) + nt * 8 * D * 2 + (j >> 1) * 128);
           mma<T>(s[nt], qh[j][0], ql[j][0], qh[j][1], ql[j][1], k.x, k.y);
-          mma<T>(s[nt], qh[j][2], ql[j][2], qh[j][3], ql[j][3], k.z, k.w);
+          mma<T>(s2[nt], qh[j][2], ql[j][2], qh[j][3], ql[j][3], k.z, k.w);
         }
       }
+      loader.issue(p, units, query_blocks, warp, s_masks[warp]);       // into the tile before's place, while the products run
       float x[4];                            // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool there = (mask >> (2 * t + (i & 1) + (i >> 1) * 8)) & 1u;
-        x[i] = there ? (s[i >> 1][i & 1] + s[i >> 1][2 + (i & 1)]) * p.scale_log2 : -INFINITY;
+        const int nt = i >> 1, e = i & 1;
+        x[i] = ((s[nt][e] + s[nt][2 + e]) + (s2[nt][e] + s2[nt][2 + e])) * p.scale_log2;
+      }
+      if (mask != 0xffffu) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((mask >> (2 * t + (i & 1) + (i >> 1) * 8)) & 1u)) x[i] = -INFINITY;
       }
       float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -503,19 +522,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       split<T>(pr[0], pr[1], ph[0], pl[0]);
       split<T>(pr[2], pr[3], ph[1], pl[1]);
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j) {
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = lds128(slot + (i & 1 ? v_odd : v_even) + (i >> 1) * 8 * D * 2 + j * 128);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t a = (&v[0].x)[e], b = (&v[1].x)[e], c = (&v[2].x)[e], d = (&v[3].x)[e];
-          mma<T>(acc[j * 8 + 2 * e], ph[0], pl[0], ph[1], pl[1], __byte_perm(a, b, 0x5410), __byte_perm(c, d, 0x5410));
-          mma<T>(acc[j * 8 + 2 * e + 1], ph[0], pl[0], ph[1], pl[1], __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x7632));
-        }
+      for (int j = 0; j < D / 16; ++j) {      // keys 0 .. 7 and 8 .. 15 of elements 16 j .. + 7, and of 16 j + 8 .. + 15
+        uint32_t v[4];
+        load_transposed(v, ((slot + v_place) ^ ((j & 3) << 5)) + (j >> 2) * 128);
+        mma<T>(acc[2 * j], ph[0], pl[0], ph[1], pl[1], v[0], v[1]);
+        mma<T>(acc[2 * j + 1], ph[0], pl[0], ph[1], pl[1], v[2], v[3]);
       }
-      __syncwarp();
-      loader.issue(p, units, query_blocks, warp, s_masks[warp]);
       stage = stage + 1 == kStages ? 0 : stage + 1;
     }
 
@@ -526,12 +538,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     if (t == 0) s_ml[warp][g] = make_float2(m, l);
     if (row_there) {
 #pragma unroll
-      for (int j = 0; j < D / 64; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {        // column 2 t of product e is element 64 j + 16 t + e, column 2 t + 1 is 8 further
-          auto of = [&](int e) { return acc[j * 8 + (i & 1) * 4 + e][i >> 1] + acc[j * 8 + (i & 1) * 4 + e][2 + (i >> 1)]; };
-          *part_at<D>(s_acc, warp, g, 16 * j + 4 * t + i) = make_float4(of(0), of(1), of(2), of(3));
-        }
+      for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
+        float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
+        *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+      }
     }
     __syncthreads();
     const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
