@@ -31,7 +31,10 @@ namespace paged {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;          // keys of a warp's step
 constexpr int kQ = 8;              // query heads of a unit; more are further units
-constexpr int kMinTiles = 8;       // a CTA's range is not made shorter: two tiles a warp
+// Tiles that a unit counts for beyond its own, where the work is divided: beginning and ending one takes a CTA about as long.  37
+// sequences of up to 1531 rows, 5 heads of 64 (units of 1 to 97 tiles): 23.2 us without, 18.0 with 4, 16.1 with 8, 16.8 with 16.
+constexpr int kUnitCost = 8;
+constexpr int kMinTiles = 8 + kUnitCost;       // a CTA's range is not made shorter: a unit of two tiles a warp
 
 struct DecodeParams {
   View q, o;                       // [B, G, H, D]
@@ -101,112 +104,107 @@ template <int D> __device__ __forceinline__ float4* part_at(float* parts, int wa
 }
 
 struct Sequence { int held, len, keys, tiles; };     // rows in the cache, with the token's own, with the depth rows; 16-key tiles (at least one)
-__device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b) {
+__device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b, bool report = false) {
   Sequence s;
-  const int room = p.pages.capacity();
-  s.held = min(max(p.pages.seq_lens[b], 0), room);
-  s.len = p.pages.seq_lens[b] >= 0 && s.held < room && p.k.ptr != nullptr ? s.held + 1 : s.held;
-  const int P = p.depth_positions != nullptr ? min(max(p.depth_positions[b], 0), p.P) : p.P;
-  const int64_t keys = (int64_t)s.len + (int64_t)P * p.L;
-  s.keys = (int)(keys < 0x7ffffff0 ? keys : 0x7ffffff0);
+  const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : p.P, own = p.k.ptr != nullptr;
+  if (report && (len < 0 || len > p.pages.room - own || seen < 0 || seen > p.P)) wrong(kBadLength);
+  s.held = min(max(len, 0), p.pages.room);
+  s.len = s.held + (len >= 0 && len < p.pages.room ? own : 0);
+  s.keys = s.len + min(max(seen, 0), p.P) * p.L;                  // below 2^31, as the tables are wide
   s.tiles = max((s.keys + kTile - 1) / kTile, 1);
   return s;
 }
-__device__ __forceinline__ void check_lengths(const DecodeParams& p, int b) {
-  const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : 0;
-  if (len < 0 || len > p.pages.capacity() - (p.k.ptr != nullptr) || seen < 0 || seen > p.P) wrong(kBadLength);
-}
 
-// A CTA's walk over its range of tiles: (sequence, unit of it, tiles [t0, t1) of the unit).
+// A CTA's walk over its range: (sequence, unit of it, tiles [t0, t1) of the unit).  A unit takes kUnitCost places before its tiles.
 struct Walk {
   int b, unit;                       // unit: head * query blocks + query block
   Sequence s;
   int t0, t1;
-  int64_t left;                      // tiles of the range from t0 on
-  __device__ __forceinline__ void cut() { t1 = (int)min((int64_t)s.tiles, t0 + left); }
+  int64_t left;                      // places of the range behind this unit
+  __device__ __forceinline__ int places() const { return s.tiles + kUnitCost; }
+  __device__ __forceinline__ void enter(int place) {
+    const int used = (int)min((int64_t)(places() - place), left);
+    left -= used;
+    t0 = max(place - kUnitCost, 0);
+    t1 = max(place + used - kUnitCost, 0);
+  }
   __device__ __forceinline__ bool next(const DecodeParams& p, int units) {
-    left -= t1 - t0;
     if (left <= 0) return false;
     if (++unit == units) { unit = 0; ++b; s = sequence(p, b); }
-    t0 = 0;
-    cut();
-    return true;
+    enter(0);
+    return t1 > 0;                   // a range may end before the unit's first tile
   }
 };
 
-// The tiles of all units in a row, divided between n CTAs: CTA i has [begin(i), begin(i + 1)).
+// The places of all units in a row, divided between n CTAs: CTA i has [begin(i), begin(i + 1)).
 struct Range {
-  int64_t total, each;               // each, and one more for some: the first `over` tiles are spread over the CTAs
+  int64_t each;                      // each, and one more for some: the first `over` are spread over the CTAs
   uint32_t n, over;
-  __device__ __forceinline__ int64_t begin(uint32_t i) const { return each * i + (n != 0 ? over * i / n : 0u); }      // over, i <= n: the product fits
+  __device__ __forceinline__ int64_t begin(uint32_t i) const { return each * i + over * i / n; }      // over, i <= n: the product fits
 };
 __device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {            // of numbers that nearly always fit 32 bits
   return (a >> 32) == 0 ? (int64_t)((uint32_t)a / b) : a / b;
 }
-// This CTA's range and where it begins.  Every warp does it by itself: a lane takes four sequences of 128 at a time.
-__device__ __forceinline__ Walk locate(const DecodeParams& p, int units, Range& r) {
-  const int lane = threadIdx.x & 31;
-  int64_t sum = 0;
-  int tiles[4];
-  auto load = [&](int base) {
+// This CTA's range, and its walk at the begin of it; at: the place of the walk's unit in the row.  False where there is nothing for it.
+__device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_tiles, Range& r, Walk& w, int64_t& at) {
+  const int tid = threadIdx.x, lane = tid & 31;
+  int sum = 0, before = 0;           // places of one unit of each sequence: below 2^31
+  int64_t begin = 0;
+  for (int pass = 0;; ++pass)        // adds them up; finds the sequence that holds `begin`
+    for (int base = 0; base < p.B; base += kThreads) {
+      if (pass == 0 || p.B > kThreads) {
+        __syncthreads();
+        s_tiles[tid] = base + tid < p.B ? sequence(p, base + tid, pass == 0 && blockIdx.x == 0).tiles + kUnitCost : 0;
+        __syncthreads();
+      }
+      const int4 x = reinterpret_cast<const int4*>(s_tiles)[lane];
+      const int mine = x.x + x.y + x.z + x.w;
+      if (pass == 0) {
+        sum += __reduce_add_sync(0xffffffffu, mine);
+        if (base + kThreads < p.B) continue;
+        const int64_t total = (int64_t)sum * units;
+        r.n = (uint32_t)min((int64_t)gridDim.x, quotient(total + kMinTiles - 1, kMinTiles));
+        if (blockIdx.x >= r.n) return false;
+        r.each = quotient(total, r.n);
+        r.over = (uint32_t)(total - r.each * r.n);
+        begin = r.begin(blockIdx.x);
+        w.left = r.begin(blockIdx.x + 1) - begin;
+        continue;
+      }
+      int incl = mine;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int b = base + lane * 4 + k;
-      tiles[k] = b < p.B ? sequence(p, b).tiles : 0;
-    }
-  };
-  for (int base = 0; base < p.B; base += 128) {
-    load(base);
-    sum += (int64_t)tiles[0] + tiles[1] + tiles[2] + tiles[3];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  r.total = sum * units;
-  r.n = (uint32_t)min((int64_t)gridDim.x, (r.total + kMinTiles - 1) / kMinTiles);
-  Walk w{};
-  if (blockIdx.x >= r.n) return w;
-  r.each = quotient(r.total, r.n);
-  r.over = (uint32_t)(r.total - r.each * r.n);
-  const int64_t begin = r.begin(blockIdx.x);
-  w.left = r.begin(blockIdx.x + 1) - begin;
-  int64_t before = 0;                                           // tiles of the sequences before this lane's first one
-  for (int base = 0;; base += 128) {
-    if (p.B > 128) load(base);
-    const int64_t mine = ((int64_t)tiles[0] + tiles[1] + tiles[2] + tiles[3]) * units;
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    const uint32_t here = __ballot_sync(0xffffffffu, begin < before + incl);
-    if (here != 0) {                                            // always at last: begin < total
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      const uint32_t here = __ballot_sync(0xffffffffu, begin < (int64_t)(before + incl) * units);
+      before += __shfl_sync(0xffffffffu, incl, 31);
+      if (here == 0) continue;
       const int from = __ffs(here) - 1;
-      int64_t off = begin - (before + incl - mine);
-      int k = 0;
-      for (; k < 3 && off >= (int64_t)tiles[k] * units; ++k) off -= (int64_t)tiles[k] * units;
-      off = __shfl_sync(0xffffffffu, off, from);
+      int first = before - __shfl_sync(0xffffffffu, incl, 31) + incl - mine, k = 0;      // of the lane's four sequences
+      if (begin >= (int64_t)(first + x.x) * units) { first += x.x; k = 1;
+        if (begin >= (int64_t)(first + x.y) * units) { first += x.y; k = 2;
+          if (begin >= (int64_t)(first + x.z) * units) { first += x.z; k = 3; } } }
+      first = __shfl_sync(0xffffffffu, first, from);
       w.b = __shfl_sync(0xffffffffu, base + lane * 4 + k, from);
       w.s = sequence(p, w.b);
-      w.unit = (int)quotient(off, (uint32_t)w.s.tiles);
-      w.t0 = (int)(off - (int64_t)w.unit * w.s.tiles);
-      w.cut();
-      return w;
+      const int64_t off = begin - (int64_t)first * units;
+      w.unit = (int)quotient(off, (uint32_t)w.places());
+      const int place = (int)(off - (int64_t)w.unit * w.places());
+      at = begin - place;
+      w.enter(place);
+      return w.t1 > w.t0;
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
 }
 // The same where a cluster of C CTAs has a unit: an even share of its tiles (none for some where there are few).
-__device__ __forceinline__ Walk locate_cluster(const DecodeParams& p, int units) {
-  Walk w{};
+__device__ __forceinline__ void locate_cluster(const DecodeParams& p, int units, Walk& w) {
   const int id = blockIdx.x / p.cluster, rank = blockIdx.x - id * p.cluster;
   w.b = id / units;
   w.unit = id - w.b * units;
-  w.s = sequence(p, w.b);
-  w.t0 = (int)((int64_t)w.s.tiles * rank / p.cluster);
-  w.t1 = (int)((int64_t)w.s.tiles * (rank + 1) / p.cluster);
-  w.left = w.t1 - w.t0;
-  return w;
+  w.s = sequence(p, w.b, w.unit == 0 && rank == 0 && threadIdx.x == 0);
+  w.t0 = (int)((uint32_t)w.s.tiles * rank / p.cluster);           // tiles below 2^27, rank below 16
+  w.t1 = (int)((uint32_t)w.s.tiles * (rank + 1) / p.cluster);
+  w.left = 0;
 }
 
 // The new token's own row of head h: turned, written to its place in the cache (page, slot) and to the copies, and the key to its
@@ -244,29 +242,30 @@ __device__ __forceinline__ void own_row(const DecodeParams& p, int b, int h, int
 }
 
 // Copies a tile's rows one by one: the ones that a page's end divides, the last ones of a sequence, its own row and the depth rows.
-// Lane l finds the K row (l < 16) or the V row of key first + l % 16, whose page is `page`.  Out of line: the loop's code stays small, and its
-// registers are not laid out for this.
+// Lane l finds the K row (l < 16) or the V row of key first + l % 16; page0 and page1: the pages of the tile's first and last key.
 template <typename T, int D>
-__device__ __noinline__ void mixed_tile(const DecodeParams& p, int b, const Sequence s, int h, bool write, int first, int page, uint32_t slot, uint32_t* mask) {
+__device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w, int h, bool write, int first, int page0, int page1, uint32_t slot, uint32_t* mask) {
   constexpr int kChunks = D / 8, kRows = 32 / kChunks, kCopies = kTile / kRows;
+  const Sequence& s = w.s;
   const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
   const int key = first + (lane & 15);
   const bool of_v = lane >= 16, own = key >= s.held && key < s.len;
-  const View &cache = of_v ? p.pages.v : p.pages.k, &depth = of_v ? p.vd : p.kd;
   bool valid = key < s.keys;
-  const unsigned char* row = static_cast<const unsigned char*>(cache.ptr);
-  int slot_of = 0;
+  const unsigned char* row = static_cast<const unsigned char*>(p.pages.k.ptr);
+  int page = -1, slot_of = 0;
   if (key < s.len) {
-    if (page >= 0 && page < p.pages.num_pages) {
-      slot_of = key - (int)p.pages.by_page.div((uint32_t)key) * p.pages.page_size;
-      row = own ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(b, 0, h) : row + 2 * cache.off(page, slot_of, h);
-    } else {
-      valid = false;
-      wrong(kBadPage);
-    }
+    const int which = (int)p.pages.by_page.div((uint32_t)key);
+    if (p.pages.page_size < kTile) page = __ldg(p.pages.table + w.b * p.pages.table_stride + which);      // a tile may lie in more than two
+    else page = which == (int)p.pages.by_page.div((uint32_t)first) ? page0 : page1;
+    slot_of = key - which * p.pages.page_size;
+    valid = page >= 0 && page < p.pages.num_pages;
+    if (!valid) wrong(kBadPage);
+    else if (own) row = static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h);
+    else row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
   } else if (valid) {
     const int d = key - s.len, pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
-    row = static_cast<const unsigned char*>(depth.ptr) + 2 * (depth.off(b, layer, h) + pos * (of_v ? p.vd_sp : p.kd_sp));
+    row = of_v ? static_cast<const unsigned char*>(p.vd.ptr) + 2 * (p.vd.off(w.b, layer, h) + pos * p.vd_sp)
+               : static_cast<const unsigned char*>(p.kd.ptr) + 2 * (p.kd.off(w.b, layer, h) + pos * p.kd_sp);
   }
   const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own && valid) & 0xffffu;
   if (lane == 0) *mask = there;
@@ -281,7 +280,7 @@ __device__ __noinline__ void mixed_tile(const DecodeParams& p, int b, const Sequ
   }
   if (its_own != 0) {
     const int n = __ffs(its_own) - 1;
-    own_row<T, D>(p, b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), s.held, write, slot, n);
+    own_row<T, D>(p, w.b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), s.held, write, slot, n);
   }
 }
 
@@ -299,51 +298,55 @@ template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to,
 template <typename T, int D> struct Loader {
   Walk w;
   int tile;                          // this warp's next one, of w
-  int page;                          // of this lane's key in it, fetched ahead
+  int base, page0, page1;            // pages of the first and the last key of this lane's tile, base + kWarps lane, fetched ahead for 32 of them
   bool more;
   uint32_t ring;
   int stage;
-  uint32_t to_k, to_v;               // where this lane's chunk of the first copy goes in a stage; the others' follow by the swizzle
+  uint32_t to_k, to_v;               // where this lane's chunk of the first copy goes in a stage
 
   static constexpr int kChunks = D / 8;
 
-  __device__ __forceinline__ void settle(const DecodeParams& p, int units, int warp) {      // at a tile of this warp, or at the end
+  __device__ __forceinline__ void settle(const DecodeParams& p, int units, int warp, bool fetch) {      // at a tile of this warp, or at the end
     while (more && tile >= w.t1) {
       more = w.next(p, units);
       tile = w.t0 + warp;
+      fetch = true;
     }
-    fetch_page(p);
-  }
-  __device__ __forceinline__ void fetch_page(const DecodeParams& p) {
-    const int key = tile * kTile + (threadIdx.x & 15);
-    page = 0;
-    if (more && key < w.s.len) page = __ldg(p.pages.table + w.b * p.pages.table_stride + p.pages.by_page.div((uint32_t)key));
+    if (!(fetch || tile == base + 32 * kWarps)) return;
+    base = tile;
+    page0 = page1 = -1;
+    const int mine = tile + kWarps * (int)(threadIdx.x & 31);
+    if (!more || mine >= w.t1 || mine * kTile >= w.s.len) return;
+    const int first = mine * kTile;
+    const int* row = p.pages.table + w.b * p.pages.table_stride;
+    page0 = __ldg(row + p.pages.by_page.div((uint32_t)first));
+    page1 = __ldg(row + p.pages.by_page.div((uint32_t)min(first + kTile, w.s.len) - 1u));
   }
   __device__ __forceinline__ void start(const DecodeParams& p, int units, int warp, const Walk& from, uint32_t ring_) {
-    w = from; more = w.left > 0; tile = w.t0 + warp; stage = 0; ring = ring_;
+    w = from; more = true; tile = w.t0 + warp; stage = 0; ring = ring_;
     const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
     to_k = r * D * 2 + (c ^ k_swizzle(r)) * 16;
     to_v = kTile * D * 2 + r * D * 2 + (c ^ r) * 16;
-    settle(p, units, warp);
+    settle(p, units, warp, true);
   }
-  // Issues the copies of one tile (none at the end); `mask` in shared memory gets a bit for each key that is there.
+  // Issues the copies of one tile (none at the end); `masks` in shared memory get a bit for each key that is there.
   __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, int warp, uint32_t* masks) {
     if (more) {
       const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
-      const int first = tile * kTile, h = w.unit / query_blocks;
+      const int first = tile * kTile, h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
       const uint32_t slot = ring + stage * stage_bytes<D>();
-      const int which = (int)p.pages.by_page.div((uint32_t)first), row0 = first - which * p.pages.page_size;
-      const int page0 = __shfl_sync(0xffffffffu, page, 0);
-      if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page0 >= 0 && page0 < p.pages.num_pages) {
+      const int row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
+      const int page = __shfl_sync(0xffffffffu, page0, (tile - base) / kWarps);
+      if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page >= 0 && page < p.pages.num_pages) {
         // sixteen rows of one page
         if (lane == 0) masks[stage] = 0xffffu;
-        copy_rows<D, false>(slot + to_k, rotary::chunk_at(p.pages.k, p.pages.k.off(page0, row0 + r, h), c), p.pages.k.st);
-        copy_rows<D, true>(slot + to_v, rotary::chunk_at(p.pages.v, p.pages.v.off(page0, row0 + r, h), c), p.pages.v.st);
+        copy_rows<D, false>(slot + to_k, rotary::chunk_at(p.pages.k, p.pages.k.off(page, row0 + r, h), c), p.pages.k.st);
+        copy_rows<D, true>(slot + to_v, rotary::chunk_at(p.pages.v, p.pages.v.off(page, row0 + r, h), c), p.pages.v.st);
       } else {
-        mixed_tile<T, D>(p, w.b, w.s, h, w.unit == h * query_blocks, first, page, slot, masks + stage);
+        mixed_tile<T, D>(p, w, h, w.unit == h * query_blocks, first, page, __shfl_sync(0xffffffffu, page1, (tile - base) / kWarps), slot, masks + stage);
       }
       tile += kWarps;
-      settle(p, units, warp);
+      settle(p, units, warp, false);
     }
     copies_commit();
     stage = stage + 1 == stages<D>() ? 0 : stage + 1;
@@ -400,87 +403,156 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   grid_started();
   Range range{};
   Walk w;
+  int64_t at = 0;                            // the place of the walk's unit in the row of all units
   if (p.cluster != 0) {
-    w = locate_cluster(p, units);
-    if (w.unit == 0 && w.t0 == 0 && tid == 0) check_lengths(p, w.b);
-  } else {
-    w = locate(p, units, range);
-    if (w.left == 0) {
-      if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
-      return;
-    }
-    if (blockIdx.x == 0)
-      for (int b = tid; b < p.B; b += kThreads) check_lengths(p, b);
+    locate_cluster(p, units, w);
+  } else if (!locate(p, units, reinterpret_cast<int*>(s_acc), range, w, at)) {
+    if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
+    return;
   }
   Loader<T, D> loader;
   loader.start(p, units, warp, w, ring);
-#pragma unroll 1
-  for (int s = 0; s < kStages - 1; ++s) loader.issue(p, units, query_blocks, warp, s_masks[warp]);
 
   // places of this lane's chunks in a stage: K of row g (even and odd j), V of row lane % 16, chunk lane / 16
   const uint32_t k_even = g * D * 2 + (t ^ k_swizzle(g)) * 16, k_odd = g * D * 2 + ((4 + t) ^ k_swizzle(g)) * 16;
   const uint32_t v_place = (kTile + lane % 16) * D * 2 + ((lane >> 4) ^ (lane & 7)) * 16;
-  int stage = 0, turned_b = -1;
-  int64_t at = range.begin(blockIdx.x);      // the walk's place in the row of all tiles
+  int stage = 0, turned_b = -1, tile = 0, h = 0, q0 = 0;
   int2 part = make_int2(0, 0);
-  bool going = true;
-  while (going) {
-    const int h = w.unit / query_blocks, q0 = (w.unit - h * query_blocks) * kQ;
-    const bool row_there = q0 + g < p.G;
-    if (p.rot.inv_freq != nullptr && turned_b != w.b) {
-      __syncthreads();
-      for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
-      __syncthreads();
-      turned_b = w.b;
-    }
-    // this lane's part of the queries, in two 16-bit halves
-    uint32_t qh[D / 32][4], ql[D / 32][4];
+  uint32_t qh[D / 32][4], ql[D / 32][4];     // this lane's part of the queries, in two 16-bit halves
+  float m = 0.f, l = 0.f, acc[D / 8][4];
+  // Steps 1 - kStages to -1 only copy.  A step's copies are issued between the scores' products and what waits for them, and at
+  // one place, for the sake of the code's size: warps are few, and wait for instructions where a step has more of them.
+  for (int step = 1 - kStages;; ++step) {
+    float s[2][4], s2[2][4];                 // two sums each: the products of one wait for one another
+    uint32_t mask = 0, slot = 0;
+    if (step >= 0) {
+      bool begins = step == 0;
+      while (begins || tile >= w.t1) {
+        if (!begins) {
+          const bool row_there = q0 + g < p.G;
+          // the warps' parts
+          l += __shfl_xor_sync(0xffffffffu, l, 1);
+          l += __shfl_xor_sync(0xffffffffu, l, 2);
+          __syncthreads();                         // the part before has been read
+          if (t == 0) s_ml[warp][g] = make_float2(m, l);
+          if (row_there) {
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const int chunk = 4 * j + t;
-      uint4 x = make_uint4(0, 0, 0, 0);
-      const int64_t row = p.q.off(w.b, q0 + g, h);
-      if (row_there) x = *rotary::chunk_at(p.q, row, chunk);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) { qh[j][e] = (&x.x)[e]; ql[j][e] = 0; }
-      if (p.rot.inv_freq != nullptr && row_there && chunk * 8 < p.rot.rot) {
-        float y[8];
-        if (p.rot.interleaved) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = Pack<T>::unpack(qh[j][e]), cs = s_cs[chunk * 4 + e];
-            y[2 * e] = fmaf(a.x, cs.x, -a.y * cs.y);
-            y[2 * e + 1] = fmaf(a.y, cs.x, a.x * cs.y);
+            for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
+              float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
+              *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+            }
           }
-        } else {
-          const int half = p.rot.rot >> 4;                     // chunks
-          const bool second = chunk >= half;
-          const uint4 other = *rotary::chunk_at(p.q, row, second ? chunk - half : chunk + half);
-          const int pair = (second ? chunk - half : chunk) * 8;
+          __syncthreads();
+          const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
+          const bool whole = p.cluster != 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
+          constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
+          const int r = tid / 16, d0 = (tid % 16) * kEach;
+          if (q0 + r < p.G) {
+            float top = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 a = Pack<T>::unpack(qh[j][e]), b = Pack<T>::unpack((&other.x)[e]);
-            const float2 c0 = s_cs[pair + 2 * e], c1 = s_cs[pair + 2 * e + 1];
-            y[2 * e] = fmaf(a.x, c0.x, second ? b.x * c0.y : -b.x * c0.y);
-            y[2 * e + 1] = fmaf(a.y, c1.x, second ? b.y * c1.y : -b.y * c1.y);
+            for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i][r].x);
+            const float base = top == -INFINITY ? 0.f : top;
+            float sum = 0.f, out[kEach] = {};
+#pragma unroll
+            for (int i = 0; i < kWarps; ++i) {
+              const float weight = fast_exp2(s_ml[i][r].x - base);
+              sum = fmaf(s_ml[i][r].y, weight, sum);
+#pragma unroll
+              for (int e = 0; e < kEach; e += 4) {
+                const float4 x = *part_at<D>(s_acc, i, r, (d0 + e) / 4);
+                out[e] = fmaf(x.x, weight, out[e]);
+                out[e + 1] = fmaf(x.y, weight, out[e + 1]);
+                out[e + 2] = fmaf(x.z, weight, out[e + 2]);
+                out[e + 3] = fmaf(x.w, weight, out[e + 3]);
+              }
+            }
+            if (whole) {
+              const float inv = sum == 0.f ? 0.f : 1.f / sum;
+              uint32_t packed[kEach / 2];
+#pragma unroll
+              for (int e = 0; e < kEach / 2; ++e) packed[e] = Pack<T>::pack(out[2 * e] * inv, out[2 * e + 1] * inv);
+              uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d0));
+#pragma unroll
+              for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
+              if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
+            } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
+              const int64_t at_row = p.cluster != 0 ? r : ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
+              float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
+#pragma unroll
+              for (int e = 0; e < kEach; ++e) to[e] = out[e];
+              if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
+            }
+          }
+          if (p.cluster != 0) {
+            if (!whole) join_cluster<T, D>(p, w, h, q0, smem_u32(smem), smem_u32(s_part_ml));
+            return;
+          }
+          if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
+            const int64_t last = at + w.places() - 1;
+            uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
+            while (range.begin(blockIdx.x + n) > last) --n;
+            while (range.begin(blockIdx.x + n + 1) <= last) ++n;
+            part = make_int2(w.b * units + w.unit, (int)n + 1);
+          }
+          at += w.places();
+          if (!w.next(p, units)) {
+            if (tid == 0) p.parts[blockIdx.x] = part;
+            return;
           }
         }
+        h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
+        q0 = (w.unit - h * query_blocks) * kQ;
+        const bool row_there = q0 + g < p.G;
+        if (p.rot.inv_freq != nullptr && turned_b != w.b) {
+          __syncthreads();
+          for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
+          __syncthreads();
+          turned_b = w.b;
+        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) split<T>(y[2 * e], y[2 * e + 1], qh[j][e], ql[j][e]);
+        for (int j = 0; j < D / 32; ++j) {
+          const int chunk = 4 * j + t;
+          uint4 x = make_uint4(0, 0, 0, 0);
+          const int64_t row = p.q.off(w.b, q0 + g, h);
+          if (row_there) x = *rotary::chunk_at(p.q, row, chunk);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { qh[j][e] = (&x.x)[e]; ql[j][e] = 0; }
+          if (p.rot.inv_freq != nullptr && row_there && chunk * 8 < p.rot.rot) {
+            float y[8];
+            if (p.rot.interleaved) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 a = Pack<T>::unpack(qh[j][e]), cs = s_cs[chunk * 4 + e];
+                y[2 * e] = fmaf(a.x, cs.x, -a.y * cs.y);
+                y[2 * e + 1] = fmaf(a.y, cs.x, a.x * cs.y);
+              }
+            } else {
+              const int half = p.rot.rot >> 4;                     // chunks
+              const bool second = chunk >= half;
+              const uint4 other = *rotary::chunk_at(p.q, row, second ? chunk - half : chunk + half);
+              const int pair = (second ? chunk - half : chunk) * 8;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 a = Pack<T>::unpack(qh[j][e]), b = Pack<T>::unpack((&other.x)[e]);
+                const float2 c0 = s_cs[pair + 2 * e], c1 = s_cs[pair + 2 * e + 1];
+                y[2 * e] = fmaf(a.x, c0.x, second ? b.x * c0.y : -b.x * c0.y);
+                y[2 * e + 1] = fmaf(a.y, c1.x, second ? b.y * c1.y : -b.y * c1.y);
+              }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) split<T>(y[2 * e], y[2 * e + 1], qh[j][e], ql[j][e]);
+          }
+        }
+        m = -INFINITY; l = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+        tile = w.t0 + warp;
+        begins = false;
       }
-    }
-
-    float m = -INFINITY, l = 0.f;
-    float acc[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-
-    for (int tile = w.t0 + warp; tile < w.t1; tile += kWarps) {
       copies_wait<kStages - 2>();
       __syncwarp();                          // the other lanes' copies, and the mask; and all lanes have read the tile before
-      const uint32_t mask = s_masks[warp][stage];
-      const uint32_t slot = ring + stage * stage_bytes<D>();
-      float s[2][4], s2[2][4];               // two sums each: the products of one wait for one another
+      mask = s_masks[warp][stage];
+      slot = ring + stage * stage_bytes<D>();
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
@@ -491,116 +563,49 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           mma<T>(s2[nt], qh[j][2], ql[j][2], qh[j][3], ql[j][3], k.z, k.w);
         }
       }
-      loader.issue(p, units, query_blocks, warp, s_masks[warp]);       // into the tile before's place, while the products run
-      float x[4];                            // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int nt = i >> 1, e = i & 1;
-        x[i] = ((s[nt][e] + s[nt][2 + e]) + (s2[nt][e] + s2[nt][2 + e])) * p.scale_log2;
-      }
-      if (mask != 0xffffu) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!((mask >> (2 * t + (i & 1) + (i >> 1) * 8)) & 1u)) x[i] = -INFINITY;
-      }
-      float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      top = fmaxf(top, m);
-      const float base = top == -INFINITY ? 0.f : top;
-      if (__any_sync(0xffffffffu, top > m)) {
-        const float shrink = fast_exp2(m - base);
-        l *= shrink;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) { acc[n][0] *= shrink; acc[n][1] *= shrink; acc[n][2] *= shrink; acc[n][3] *= shrink; }
-        m = top;
-      }
-      float pr[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { pr[i] = fast_exp2(x[i] - base); l += pr[i]; }
-      uint32_t ph[2], pl[2];
-      split<T>(pr[0], pr[1], ph[0], pl[0]);
-      split<T>(pr[2], pr[3], ph[1], pl[1]);
-#pragma unroll
-      for (int j = 0; j < D / 16; ++j) {      // keys 0 .. 7 and 8 .. 15 of elements 16 j .. + 7, and of 16 j + 8 .. + 15
-        uint32_t v[4];
-        load_transposed(v, ((slot + v_place) ^ ((j & 3) << 5)) + (j >> 2) * 128);
-        mma<T>(acc[2 * j], ph[0], pl[0], ph[1], pl[1], v[0], v[1]);
-        mma<T>(acc[2 * j + 1], ph[0], pl[0], ph[1], pl[1], v[2], v[3]);
-      }
-      stage = stage + 1 == kStages ? 0 : stage + 1;
     }
-
-    // the warps' parts
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
-    __syncthreads();                         // the part before has been read
-    if (t == 0) s_ml[warp][g] = make_float2(m, l);
-    if (row_there) {
+    loader.issue(p, units, query_blocks, warp, s_masks[warp]);
+    if (step < 0) continue;
+    float x[4];                            // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
-        float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
-        *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      const int nt = i >> 1, e = i & 1;
+      x[i] = ((s[nt][e] + s[nt][2 + e]) + (s2[nt][e] + s2[nt][2 + e])) * p.scale_log2;
     }
-    __syncthreads();
-    const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
-    const bool whole = p.cluster != 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
-    constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
-    const int r = tid / 16, d0 = (tid % 16) * kEach;
-    if (q0 + r < p.G) {
-      float top = -INFINITY;
+    if (mask != 0xffffu) {
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i][r].x);
-      const float base = top == -INFINITY ? 0.f : top;
-      float sum = 0.f, out[kEach] = {};
-#pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        const float weight = fast_exp2(s_ml[i][r].x - base);
-        sum = fmaf(s_ml[i][r].y, weight, sum);
-#pragma unroll
-        for (int e = 0; e < kEach; e += 4) {
-          const float4 x = *part_at<D>(s_acc, i, r, (d0 + e) / 4);
-          out[e] = fmaf(x.x, weight, out[e]);
-          out[e + 1] = fmaf(x.y, weight, out[e + 1]);
-          out[e + 2] = fmaf(x.z, weight, out[e + 2]);
-          out[e + 3] = fmaf(x.w, weight, out[e + 3]);
-        }
-      }
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint32_t packed[kEach / 2];
-#pragma unroll
-        for (int e = 0; e < kEach / 2; ++e) packed[e] = Pack<T>::pack(out[2 * e] * inv, out[2 * e + 1] * inv);
-        uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d0));
-#pragma unroll
-        for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
-        if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
-      } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
-        const int64_t at_row = p.cluster != 0 ? r : ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
-        float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) to[e] = out[e];
-        if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
-      }
+      for (int i = 0; i < 4; ++i)
+        if (!((mask >> (2 * t + (i & 1) + (i >> 1) * 8)) & 1u)) x[i] = -INFINITY;
     }
-    if (p.cluster != 0) {
-      if (!whole) join_cluster<T, D>(p, w, h, q0, smem_u32(smem), smem_u32(s_part_ml));
-      return;
+    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    top = fmaxf(top, m);
+    const float base = top == -INFINITY ? 0.f : top;
+    if (__any_sync(0xffffffffu, top > m)) {
+      const float shrink = fast_exp2(m - base);
+      l *= shrink;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) { acc[n][0] *= shrink; acc[n][1] *= shrink; acc[n][2] *= shrink; acc[n][3] *= shrink; }
+      m = top;
     }
-    if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
-      const int64_t last = at + w.s.tiles - 1;
-      uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
-      while (range.begin(blockIdx.x + n) > last) --n;
-      while (range.begin(blockIdx.x + n + 1) <= last) ++n;
-      part = make_int2(w.b * units + w.unit, (int)n + 1);
+    float pr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { pr[i] = fast_exp2(x[i] - base); l += pr[i]; }
+    uint32_t ph[2], pl[2];
+    split<T>(pr[0], pr[1], ph[0], pl[0]);
+    split<T>(pr[2], pr[3], ph[1], pl[1]);
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {      // keys 0 .. 7 and 8 .. 15 of elements 16 j .. + 7, and of 16 j + 8 .. + 15
+      uint32_t v[4];
+      load_transposed(v, ((slot + v_place) ^ ((j & 3) << 5)) + (j >> 2) * 128);
+      mma<T>(acc[2 * j], ph[0], pl[0], ph[1], pl[1], v[0], v[1]);
+      mma<T>(acc[2 * j + 1], ph[0], pl[0], ph[1], pl[1], v[2], v[3]);
     }
-    at += w.t1 - w.t0;
-    going = w.next(p, units);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    tile += kWarps;
   }
-  if (tid == 0) p.parts[blockIdx.x] = part;
 }
-
 // Joins the parts of the units that several CTAs hold.  Grid: (CTA in which the unit begins, query row).
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ DecodeParams p) {

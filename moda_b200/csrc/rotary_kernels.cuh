@@ -182,10 +182,7 @@ struct Pages {
   const int* seq_lens;       // [B]
   int num_pages, page_size, max_pages;
   FastDiv by_page;
-  __device__ __forceinline__ int capacity() const {           // positions that a row of the table covers
-    const int64_t n = (int64_t)max_pages * page_size;
-    return n < 0x7fffffff ? (int)n : 0x7fffffff;
-  }
+  int room;                  // positions that a row of the table covers, at most 2^31 - 1
 };
 
 // What a call found wrong in its tables or lengths: 2 << 8 | one of these, kept until the host reads it.  The
@@ -218,7 +215,7 @@ __global__ void __launch_bounds__(rotary::kThreads) append_kernel(const __grid_c
     const int b = (int)p.by_t.div((uint32_t)tok), t = (int)(tok - (int64_t)b * p.T);
     if (p.lengths != nullptr && t >= p.lengths[b]) continue;
     const int64_t n = (int64_t)p.pages.seq_lens[b] + t;
-    if (n < 0 || n >= p.pages.capacity()) {
+    if (n < 0 || n >= p.pages.room) {
       if (lane == 0) wrong(kBadLength);
       continue;
     }

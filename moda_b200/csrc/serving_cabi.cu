@@ -45,6 +45,7 @@ int check_pages(const moda_problem* pr, const moda_paged_cache* c, paged::Pages*
   out->k = to_view(&c->k); out->v = to_view(&c->v);
   out->table = c->block_table; out->table_stride = c->table_stride; out->seq_lens = c->seq_lens;
   out->num_pages = c->num_pages; out->page_size = c->page_size; out->max_pages = c->max_pages;
+  out->room = (int)std::min<int64_t>((int64_t)c->max_pages * c->page_size, 0x7fffffff);
   out->by_page = rotary::FastDiv((uint32_t)c->page_size);
   return MODA_OK;
 }
@@ -95,7 +96,7 @@ Division divide(const moda_problem* pr, int64_t most_keys, int n_sm) {
   int cluster = 1;
   while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
   if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
-  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, units * tiles / paged::kMinTiles)), 0};
+  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, (units * (tiles + paged::kUnitCost) + paged::kMinTiles - 1) / paged::kMinTiles)), 0};
 }
 // Scratch of an evenly divided call: which units are shared, their parts' maxima and sums, their parts.
 size_t parts_bytes(int n) { return ((size_t)n * sizeof(int2) + 255) & ~(size_t)255; }
@@ -260,11 +261,14 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   } else if (prob->L > 0) {
     return MODA_ERR_NULL;
   }
+  // the kernels count keys, and the tiles of one head of all sequences, in 31 bits
+  const int64_t most_keys = (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L;
+  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 1 + paged::kUnitCost) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  const Division div = divide(prob, (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L, n_sm);
+  const Division div = divide(prob, most_keys, n_sm);
   const int n_cta = div.ctas;
   p.cluster = div.cluster;
   if (workspace == nullptr || workspace_bytes < decode_scratch(2 * n_sm, prob->D)) return MODA_ERR_WORKSPACE;
