@@ -400,6 +400,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
   float* s_acc = reinterpret_cast<float*>(smem + (size_t)kWarps * kStages * stage_bytes<D>());
 
+  grid_before();
   grid_started();
   Range range{};
   Walk w;
@@ -420,8 +421,25 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   int2 part = make_int2(0, 0);
   uint32_t qh[D / 32][4], ql[D / 32][4];     // this lane's part of the queries, in two 16-bit halves
   float m = 0.f, l = 0.f, acc[D / 8][4];
+  const double inv_freq = p.rot.inv_freq != nullptr && tid < p.rot.rot / 2 ? p.rot.inv_freq[tid] : 0.;
+  // What a unit begins with: its queries' rows, and cosines and sines of their position, one a thread (those of the unit before have been
+  // read: its parts have been joined).
+  auto fetch = [&]() {
+    h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
+    q0 = (w.unit - h * query_blocks) * kQ;
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) {
+      uint4 x = make_uint4(0, 0, 0, 0);
+      if (q0 + g < p.G) x = *rotary::chunk_at(p.q, p.q.off(w.b, q0 + g, h), 4 * j + t);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qh[j][e] = (&x.x)[e];
+    }
+    if (tid < p.rot.rot / 2 && turned_b != w.b) s_cs[tid] = rotary::cos_sin(p.rot, inv_freq, p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
+    turned_b = w.b;
+  };
   // Steps 1 - kStages to -1 only copy.  A step's copies are issued between the scores' products and what waits for them, and at
   // one place, for the sake of the code's size: warps are few, and wait for instructions where a step has more of them.
+  fetch();
   for (int step = 1 - kStages;; ++step) {
     float s[2][4], s2[2][4];                 // two sums each: the products of one wait for one another
     uint32_t mask = 0, slot = 0;
@@ -500,23 +518,15 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
             return;
           }
         }
-        h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
-        q0 = (w.unit - h * query_blocks) * kQ;
+        if (step > 0) fetch();
         const bool row_there = q0 + g < p.G;
-        if (p.rot.inv_freq != nullptr && turned_b != w.b) {
-          __syncthreads();
-          for (int i = tid; i < p.rot.rot / 2; i += kThreads) s_cs[i] = rotary::cos_sin(p.rot, p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
-          __syncthreads();
-          turned_b = w.b;
-        }
+        if (p.rot.inv_freq != nullptr) __syncthreads();
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const int chunk = 4 * j + t;
-          uint4 x = make_uint4(0, 0, 0, 0);
           const int64_t row = p.q.off(w.b, q0 + g, h);
-          if (row_there) x = *rotary::chunk_at(p.q, row, chunk);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) { qh[j][e] = (&x.x)[e]; ql[j][e] = 0; }
+          for (int e = 0; e < 4; ++e) ql[j][e] = 0;
           if (p.rot.inv_freq != nullptr && row_there && chunk * 8 < p.rot.rot) {
             float y[8];
             if (p.rot.interleaved) {
@@ -606,11 +616,13 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     tile += kWarps;
   }
 }
-// Joins the parts of the units that several CTAs hold.  Grid: (CTA in which the unit begins, query row).
+// Joins the parts of the units that several CTAs hold.  Grid: (CTA in which the unit begins, query row).  A warp takes every eighth
+// part, five of them on the way together: 40 parts, what one sequence with 8 heads has, take one trip to memory.
+constexpr int kJoinWarps = 8, kJoinAhead = 5;
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ float s_acc[kWarps][D];
-  __shared__ float2 s_ml[kWarps];
+__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ float s_acc[kJoinWarps][D];
+  __shared__ float2 s_ml[kJoinWarps];
   grid_before();
   const int2 part = p.parts[blockIdx.x];
   const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
@@ -620,37 +632,46 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   auto place = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
   constexpr int kEach = D / 32;
   float top = -INFINITY, sum = 0.f, out[kEach] = {};
-#pragma unroll 4
-  for (int i = warp; i < part.y; i += kWarps) {
-    const float2 ml = p.ml[place(i)];
-    float x[kEach];
+  for (int i0 = warp; i0 < part.y; i0 += kJoinAhead * kJoinWarps) {
+    float2 ml[kJoinAhead];
+    float x[kJoinAhead][kEach];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) x[e] = p.acc[place(i) * D + lane * kEach + e];
-    const float now = fmaxf(top, ml.x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(ml.x - base);
-    sum = sum * a + ml.y * b;
+    for (int k = 0; k < kJoinAhead; ++k) {
+      const int64_t at = place(min(i0 + k * kJoinWarps, part.y - 1));      // beyond the last one: it again, unused
+      ml[k] = p.ml[at];
+      const float* from = p.acc + at * D + lane * kEach;
+      if constexpr (kEach == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
+      else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
+    }
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) out[e] = out[e] * a + x[e] * b;
-    top = now;
+    for (int k = 0; k < kJoinAhead; ++k) {
+      if (i0 + k * kJoinWarps >= part.y) break;
+      const float now = fmaxf(top, ml[k].x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(ml[k].x - base);
+      sum = sum * a + ml[k].y * b;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) out[e] = out[e] * a + x[k][e] * b;
+      top = now;
+    }
   }
 #pragma unroll
   for (int e = 0; e < kEach; ++e) s_acc[warp][lane * kEach + e] = out[e];
   if (lane == 0) s_ml[warp] = make_float2(top, sum);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i].x);
+  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, s_ml[i].x);
   const float base = top == -INFINITY ? 0.f : top;
-  float weight[kWarps];
+  float weight[kJoinWarps];
   sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
+  for (int i = 0; i < kJoinWarps; ++i) {
     weight[i] = fast_exp2(s_ml[i].x - base);
     sum = fmaf(s_ml[i].y, weight[i], sum);
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = threadIdx.x; d < D / 2; d += kThreads) {
+  for (int d = threadIdx.x; d < D / 2; d += kJoinWarps * 32) {
     float x = 0.f, y = 0.f;
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) { x = fmaf(s_acc[i][2 * d], weight[i], x); y = fmaf(s_acc[i][2 * d + 1], weight[i], y); }
+    for (int i = 0; i < kJoinWarps; ++i) { x = fmaf(s_acc[i][2 * d], weight[i], x); y = fmaf(s_acc[i][2 * d + 1], weight[i], y); }
     reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * p.o.off(b, row, h))[d] = Pack<T>::pack(x * inv, y * inv);
   }
   if (threadIdx.x == 0) p.lse[((int64_t)b * p.G + row) * p.H + h] = top + log2f(sum);

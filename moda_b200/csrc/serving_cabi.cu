@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "cabi_common.cuh"
 #include "profiler.cuh"
@@ -103,22 +104,31 @@ size_t parts_bytes(int n) { return ((size_t)n * sizeof(int2) + 255) & ~(size_t)2
 size_t ml_bytes(int n) { return (size_t)n * 2 * paged::kQ * sizeof(float2); }
 size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * 2 * paged::kQ * D * sizeof(float); }
 
-template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, cudaStream_t st) {
+template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, int device, cudaStream_t st) {
   auto kern = paged::decode_kernel<T, D>;
   constexpr size_t smem = paged::smem_bytes<D>();
-  if (int rc = opt_in_smem(kern, smem)) return rc;
-  cudaLaunchAttribute attr{};
+  // once a device (the call costs the host 0.4 us)
+  static std::atomic<uint64_t> prepared{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
+    if (int rc = opt_in_smem(kern, smem)) return rc;
+    MODA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    prepared.fetch_or(bit, std::memory_order_relaxed);
+  }
+  // The launch may begin when the grid before it has ended but not flushed what it wrote: the kernel waits for that itself.
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = std::max(p.cluster, 1);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(n_cta);
   cfg.blockDim = dim3(paged::kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cfg.attrs = &attr;
-  cfg.numAttrs = p.cluster > 1 ? 1 : 0;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = std::max(p.cluster, 1);
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  if (p.cluster > 8) MODA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   cudaError_t e;
   {
     prof::Scope ps(prof::kPagedDecode, st);
@@ -128,11 +138,9 @@ template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta,
   g_last_launches += 1;
   if (p.cluster != 0) return MODA_OK;
   cfg.gridDim = dim3(n_cta, std::min(p.G, paged::kQ));
+  cfg.blockDim = dim3(paged::kJoinWarps * 32);
   cfg.dynamicSmemBytes = 0;
   cfg.numAttrs = 1;
-  attr = cudaLaunchAttribute{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
   {
     prof::Scope ps(prof::kPagedJoin, st);
     e = cudaLaunchKernelEx(&cfg, paged::join_kernel<T, D>, p);
@@ -285,8 +293,8 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   g_last_launches = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = prob->dtype == MODA_BF16;
-  if (prob->D == 128) return bf ? decode<__nv_bfloat16, 128>(p, n_cta, st) : decode<__half, 128>(p, n_cta, st);
-  return bf ? decode<__nv_bfloat16, 64>(p, n_cta, st) : decode<__half, 64>(p, n_cta, st);
+  if (prob->D == 128) return bf ? decode<__nv_bfloat16, 128>(p, n_cta, prob->device, st) : decode<__half, 128>(p, n_cta, prob->device, st);
+  return bf ? decode<__nv_bfloat16, 64>(p, n_cta, prob->device, st) : decode<__half, 64>(p, n_cta, prob->device, st);
 }
 
 }  // extern "C"
