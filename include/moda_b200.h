@@ -281,9 +281,11 @@ int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, cons
  * Rows in pages that are none of the pool's are left out and recorded, as are lengths that are negative or
  * more than the table covers.
  * The results do not depend on scheduling.  workspace: caller-owned DEVICE scratch, 256-byte aligned,
- * contents undefined on entry and exit; calls that may overlap on the GPU need one each.
+ * contents undefined on entry and exit; calls that may overlap on the GPU need one each.  How many bytes (0: none, and
+ * workspace may be NULL) depends on B, H, G, D and on how long the table lets a sequence be (max_pages, page_size).
  */
-int moda_b200_paged_decode_workspace_bytes(const moda_problem *prob, size_t *bytes);
+int moda_b200_paged_decode_workspace_bytes(const moda_problem *prob, const moda_paged_cache *cache,
+                                           size_t *bytes);
 int moda_b200_paged_decode(const moda_problem *prob, const moda_tensor4 *q, const moda_paged_cache *cache,
                            const moda_tensor4 *k, const moda_tensor4 *v, const moda_tensor4 *k_copy,
                            const moda_tensor4 *v_copy, const moda_depth_rows *depth, const moda_rotary *rot,

@@ -135,7 +135,7 @@ def load() -> ctypes.CDLL:
     lib.moda_b200_rotary.restype = ctypes.c_int
     lib.moda_b200_paged_append.argtypes = [P, T, T, C, V, R, V]
     lib.moda_b200_paged_append.restype = ctypes.c_int
-    lib.moda_b200_paged_decode_workspace_bytes.argtypes = [P, ctypes.POINTER(ctypes.c_size_t)]
+    lib.moda_b200_paged_decode_workspace_bytes.argtypes = [P, C, ctypes.POINTER(ctypes.c_size_t)]
     lib.moda_b200_paged_decode_workspace_bytes.restype = ctypes.c_int
     lib.moda_b200_paged_decode.argtypes = [P, T, C, T, T, T, T, W, R, T, V, V, ctypes.c_size_t, V]
     lib.moda_b200_paged_decode.restype = ctypes.c_int

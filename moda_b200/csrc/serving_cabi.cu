@@ -60,15 +60,33 @@ dim3 token_grid(int64_t tokens, int vectors, int D, int n_sm, int* per_warp) {
   const int64_t shares = std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)n_sm * 16 / std::max<int64_t>(tokens, 1)));
   const int steps = (int)((most + shares - 1) / shares);
   *per_warp = steps * step;
-  const int64_t blocks = (tokens + warps - 1) / warps;
-  return dim3((unsigned)std::min<int64_t>(blocks, (int64_t)n_sm * 64), (unsigned)((vectors + *per_warp - 1) / *per_warp));
+  return dim3((unsigned)((tokens + warps - 1) / warps), (unsigned)((vectors + *per_warp - 1) / *per_warp));
 }
 
-template <typename T, int D> void launch_rotary(const rotary::RotaryParams& p, dim3 grid, cudaStream_t st) {
-  rotary::rotary_kernel<T, D><<<grid, rotary::kThreads, 0, st>>>(p);
+// A launch that may begin when the grid before it has ended but not flushed what it wrote: the kernels here wait for that themselves, before
+// anything else.  A cluster of `cluster` CTAs.
+template <typename P>
+cudaError_t launch(void (*kern)(P), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const P& p) {
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, p);
 }
-template <typename T, int D> void launch_append(const paged::AppendParams& p, dim3 grid, cudaStream_t st) {
-  paged::append_kernel<T, D><<<grid, rotary::kThreads, 0, st>>>(p);
+template <typename T, int D> cudaError_t launch_rotary(const rotary::RotaryParams& p, dim3 grid, cudaStream_t st) {
+  return launch(rotary::rotary_kernel<T, D>, grid, rotary::kThreads, 0, 1, st, p);
+}
+template <typename T, int D> cudaError_t launch_append(const paged::AppendParams& p, dim3 grid, cudaStream_t st) {
+  return launch(paged::append_kernel<T, D>, grid, rotary::kThreads, 0, 1, st, p);
 }
 
 int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v, const paged::Pages& pages, const int32_t* lengths,
@@ -77,13 +95,14 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
   p.k = to_view(k); p.v = to_view(v); p.pages = pages; p.lengths = lengths; p.rot = rot;
   p.B = pr->B; p.T = pr->T_kv; p.H = pr->H; p.by_t = rotary::FastDiv((uint32_t)pr->T_kv);
   const dim3 grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm, &p.per_warp);
+  cudaError_t e;
   {
     prof::Scope ps(prof::kPagedAppend, st);
     const bool bf = pr->dtype == MODA_BF16;
-    if (pr->D == 128) bf ? launch_append<__nv_bfloat16, 128>(p, grid, st) : launch_append<__half, 128>(p, grid, st);
-    else bf ? launch_append<__nv_bfloat16, 64>(p, grid, st) : launch_append<__half, 64>(p, grid, st);
+    if (pr->D == 128) e = bf ? launch_append<__nv_bfloat16, 128>(p, grid, st) : launch_append<__half, 128>(p, grid, st);
+    else e = bf ? launch_append<__nv_bfloat16, 64>(p, grid, st) : launch_append<__half, 64>(p, grid, st);
   }
-  MODA_CUDA(cudaGetLastError());
+  MODA_CUDA(e);
   g_last_launches += 1;
   return MODA_OK;
 }
@@ -91,9 +110,9 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
 // How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
 // the width of its table.
 struct Division { int ctas, cluster; };
-Division divide(const moda_problem* pr, int64_t most_keys, int n_sm) {
+Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
   const int64_t heads = (int64_t)pr->H * ((pr->G + paged::kQ - 1) / paged::kQ), units = pr->B * heads;
-  const int64_t tiles = std::max<int64_t>(1, (most_keys + paged::kTile - 1) / paged::kTile), slots = 2 * n_sm;
+  const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile), slots = 2 * n_sm;
   int cluster = 1;
   while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
   if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
@@ -115,35 +134,17 @@ template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta,
     MODA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     prepared.fetch_or(bit, std::memory_order_relaxed);
   }
-  // The launch may begin when the grid before it has ended but not flushed what it wrote: the kernel waits for that itself.
-  cudaLaunchAttribute attr[2]{};
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = std::max(p.cluster, 1);
-  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(n_cta);
-  cfg.blockDim = dim3(paged::kThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.cluster > 1 ? 2 : 1;
   cudaError_t e;
   {
     prof::Scope ps(prof::kPagedDecode, st);
-    e = cudaLaunchKernelEx(&cfg, kern, p);
+    e = launch(kern, dim3(n_cta), paged::kThreads, smem, std::max(p.cluster, 1), st, p);
   }
   MODA_CUDA(e);
   g_last_launches += 1;
   if (p.cluster != 0) return MODA_OK;
-  cfg.gridDim = dim3(n_cta, std::min(p.G, paged::kQ));
-  cfg.blockDim = dim3(paged::kJoinWarps * 32);
-  cfg.dynamicSmemBytes = 0;
-  cfg.numAttrs = 1;
   {
     prof::Scope ps(prof::kPagedJoin, st);
-    e = cudaLaunchKernelEx(&cfg, paged::join_kernel<T, D>, p);
+    e = launch(paged::join_kernel<T, D>, dim3(n_cta, std::min(p.G, paged::kQ)), paged::kJoinWarps * 32, 0, 1, st, p);
   }
   MODA_CUDA(e);
   g_last_launches += 1;
@@ -195,13 +196,14 @@ int moda_b200_rotary(const moda_problem* prob, const moda_rotary* rot, const mod
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const dim3 grid = token_grid(B * T, p.vectors, prob->D, n_sm, &p.per_warp);
+  cudaError_t e;
   {
     prof::Scope ps(prof::kRotary, st);
     const bool bf = prob->dtype == MODA_BF16;
-    if (prob->D == 128) bf ? launch_rotary<__nv_bfloat16, 128>(p, grid, st) : launch_rotary<__half, 128>(p, grid, st);
-    else bf ? launch_rotary<__nv_bfloat16, 64>(p, grid, st) : launch_rotary<__half, 64>(p, grid, st);
+    if (prob->D == 128) e = bf ? launch_rotary<__nv_bfloat16, 128>(p, grid, st) : launch_rotary<__half, 128>(p, grid, st);
+    else e = bf ? launch_rotary<__nv_bfloat16, 64>(p, grid, st) : launch_rotary<__half, 64>(p, grid, st);
   }
-  MODA_CUDA(cudaGetLastError());
+  MODA_CUDA(e);
   g_last_launches += 1;
   return MODA_OK;
 }
@@ -224,12 +226,14 @@ int moda_b200_paged_append(const moda_problem* prob, const moda_tensor4* k, cons
   return append(prob, k, v, pages, lengths, turn, n_sm, reinterpret_cast<cudaStream_t>(stream));
 }
 
-int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, size_t* bytes) {
-  if (bytes == nullptr) return MODA_ERR_NULL;
+int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, const moda_paged_cache* cache, size_t* bytes) {
+  if (bytes == nullptr || cache == nullptr) return MODA_ERR_NULL;
   if (int rc = check_sizes(prob)) return rc;
+  if (cache->max_pages < 1 || cache->page_size < 1) return MODA_ERR_SHAPE;
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  *bytes = decode_scratch(2 * n_sm, prob->D);
+  const Division div = divide(prob, (int64_t)cache->max_pages * cache->page_size, n_sm);
+  *bytes = div.cluster != 0 ? 0 : decode_scratch(div.ctas, prob->D);
   return MODA_OK;
 }
 
@@ -276,11 +280,13 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   if (!guard.ok) return cuda_fail(guard.err);
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  const Division div = divide(prob, most_keys, n_sm);
+  const Division div = divide(prob, (int64_t)p.pages.max_pages * p.pages.page_size, n_sm);
   const int n_cta = div.ctas;
   p.cluster = div.cluster;
-  if (workspace == nullptr || workspace_bytes < decode_scratch(2 * n_sm, prob->D)) return MODA_ERR_WORKSPACE;
-  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
+  if (p.cluster == 0) {
+    if (workspace == nullptr || workspace_bytes < decode_scratch(n_cta, prob->D)) return MODA_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
+  }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.q = to_view(q); p.o = to_view(o); p.lse = lse;
   p.B = prob->B; p.H = prob->H; p.G = prob->G;

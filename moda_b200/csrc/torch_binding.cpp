@@ -824,11 +824,11 @@ PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     r.o = at::empty(q.sizes(), q.options());
     r.lse = at::empty({B, G, H}, q.options().dtype(at::kFloat));
     size_t bytes = 0;
-    check_status(moda_b200_paged_decode_workspace_bytes(&pr, &bytes), "moda_b200_paged_decode_workspace_bytes");
-    const Tensor ws = at::empty({(int64_t)bytes}, q.options().dtype(at::kByte));
+    check_status(moda_b200_paged_decode_workspace_bytes(&pr, &c.abi, &bytes), "moda_b200_paged_decode_workspace_bytes");
+    const Tensor ws = bytes > 0 ? at::empty({(int64_t)bytes}, q.options().dtype(at::kByte)) : Tensor();
     check_status(moda_b200_paged_decode(&pr, T4(q).p(), &c.abi, T4(k).p(), T4(v).p(), T4(rk).p(), T4(rv).p(), L > 0 ? &depth : nullptr,
                                         spec.inv_freq.defined() ? &rot : nullptr, T4(r.o).p(), r.lse.mutable_data_ptr<float>(),
-                                        ws.mutable_data_ptr(), bytes, c10::cuda::getCurrentCUDAStream().stream()),
+                                        bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream().stream()),
                  "moda_b200_paged_decode");
   }
   return wrap(r);

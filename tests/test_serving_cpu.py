@@ -183,7 +183,7 @@ def test_c_abi_refusals(built_library):
     assert decode(p=prob(L=3), depth=rows(positions_per_sequence=0)) == 2 and decode(p=prob(L=3), depth=rows(k=null)) == 1
     assert decode(p=prob(L=3), depth=rows(k_stride_position=0)) == 5 and decode(p=prob(L=3), depth=rows(positions_seen=0x1001)) == 5
     assert decode(p=prob(L=1 << 20), depth=rows(positions_per_sequence=1 << 20)) == 2
-    assert lib.moda_b200_paged_decode_workspace_bytes(r(prob()), None) == 1
+    assert lib.moda_b200_paged_decode_workspace_bytes(r(prob()), r(pages()), None) == 1
 
 
 @pytest.mark.parametrize("rot", [16, 48, 64, 128])
