@@ -517,8 +517,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
             if (tid == 0) p.parts[blockIdx.x] = part;
             return;
           }
+          fetch();
         }
-        if (step > 0) fetch();
         const bool row_there = q0 + g < p.G;
         if (p.rot.inv_freq != nullptr) __syncthreads();
 #pragma unroll

@@ -60,6 +60,13 @@ DECODE = [  # dtype, lengths, H, G, D, L, page, heads
     (HF, [20000, 1], 1, 2, 64, 1, 128, True),
     (BF, list(range(0, 290, 2)), 2, 2, 64, 5, 32, True),       # more sequences than a CTA has threads
     (BF, [33], 200, 1, 64, 2, 256, False),
+    # more heads than CTAs: the work is divided evenly, whatever it is made of
+    (HF, [(37 * i) % 301 for i in range(80)], 5, 3, 64, 4, 16, True),
+    (BF, [(53 * i) % 900 for i in range(70)], 5, 4, 128, 7, 64, True),
+    (BF, [0, 1, 15, 16, 17, 4000] * 12, 6, 2, 128, 0, 24, False),
+    (HF, [2500, 0, 3, 900], 5, 9, 128, 2, 32, True),           # few heads, too long for clusters
+    (BF, [9000, 8999], 8, 8, 64, 11, 256, True),
+    (BF, [1] * 1000, 3, 1, 64, 0, 8, True),
 ]
 
 
