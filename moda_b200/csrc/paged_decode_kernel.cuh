@@ -31,10 +31,14 @@ namespace paged {
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kTile = 16;          // keys of a warp's step
 constexpr int kQ = 8;              // query heads of a unit; more are further units
+// A team takes a unit: the four warps of a CTA, which divide its tiles; or, where there are many short units (kShort tiles on average),
+// each warp by itself, which has nothing to wait for.  1708 units of one tile, D = 128: 37 us by CTAs, 21 by warps.
+constexpr int kShort = 12;
 // Tiles that a unit counts for beyond its own, where the work is divided: beginning and ending one takes a CTA about as long.  37
 // sequences of up to 1531 rows, 5 heads of 64 (units of 1 to 97 tiles): 23.2 us without, 18.0 with 4, 16.1 with 8, 16.8 with 16.
-constexpr int kUnitCost = 8;
-constexpr int kMinTiles = 8 + kUnitCost;       // a CTA's range is not made shorter: a unit of two tiles a warp
+__host__ __device__ constexpr int unit_cost(int team) { return team == 1 ? 2 : 8; }
+// A range is not made shorter: a unit of two tiles a warp.
+__host__ __device__ constexpr int least_places(int team) { return 2 * team + unit_cost(team); }
 
 struct DecodeParams {
   View q, o;                       // [B, G, H, D]
@@ -52,9 +56,10 @@ struct DecodeParams {
   float scale_log2;
   int cluster;                     // 0: units are divided evenly over all CTAs; C: each unit over the C CTAs of a cluster
   // scratch where units are divided over all CTAs
-  int2* parts;                     // [CTA]: unit that is begun there and goes on in the next ones, and in how many it lies (0: none)
-  float2* ml;                      // [CTA][2][kQ]: maximum and sum; part 0 goes on from the CTA before, part 1 begins here
-  float* acc;                      // [CTA][2][kQ][D]
+  int2* parts;                     // [kWarps][CTA], of a CTA's one team or four: unit that it begins and others go on with, and how many hold a part
+                                   // (none: 0; with four teams the numbers are negative, none: -1)
+  float2* ml;                      // [team][2][kQ]: maximum and sum; part 0 goes on from the team before, part 1 begins here
+  float* acc;                      // [team][2][kQ][D]
 };
 
 template <typename T> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -115,18 +120,19 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b, bool 
   return s;
 }
 
-// A CTA's walk over its range: (sequence, unit of it, tiles [t0, t1) of the unit).  A unit takes kUnitCost places before its tiles.
+// A team's walk over its range: (sequence, unit of it, tiles [t0, t1) of the unit).  A unit takes `cost` places before its tiles.
 struct Walk {
+  int cost;
   int b, unit;                       // unit: head * query blocks + query block
   Sequence s;
   int t0, t1;
   int64_t left;                      // places of the range behind this unit
-  __device__ __forceinline__ int places() const { return s.tiles + kUnitCost; }
+  __device__ __forceinline__ int places() const { return s.tiles + cost; }
   __device__ __forceinline__ void enter(int place) {
     const int used = (int)min((int64_t)(places() - place), left);
     left -= used;
-    t0 = max(place - kUnitCost, 0);
-    t1 = max(place + used - kUnitCost, 0);
+    t0 = max(place - cost, 0);
+    t1 = max(place + used - cost, 0);
   }
   __device__ __forceinline__ bool next(const DecodeParams& p, int units) {
     if (left <= 0) return false;
@@ -136,41 +142,51 @@ struct Walk {
   }
 };
 
-// The places of all units in a row, divided between n CTAs: CTA i has [begin(i), begin(i + 1)).
+// The places of all units in a row, divided between n teams: team i has [begin(i), begin(i + 1)).
 struct Range {
-  int64_t each;                      // each, and one more for some: the first `over` are spread over the CTAs
+  int64_t each;                      // each, and one more for some: the first `over` are spread over the teams
   uint32_t n, over;
   __device__ __forceinline__ int64_t begin(uint32_t i) const { return each * i + over * i / n; }      // over, i <= n: the product fits
 };
 __device__ __forceinline__ int64_t quotient(int64_t a, uint32_t b) {            // of numbers that nearly always fit 32 bits
   return (a >> 32) == 0 ? (int64_t)((uint32_t)a / b) : a / b;
 }
-// This CTA's range, and its walk at the begin of it; at: the place of the walk's unit in the row.  False where there is nothing for it.
-__device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_tiles, Range& r, Walk& w, int64_t& at) {
+// The team's size and range, and its walk at the begin of it; at: the place of the walk's unit in the row.  False where there is nothing for it.
+__device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_tiles, int& team, Range& r, Walk& w, int64_t& at) {
   const int tid = threadIdx.x, lane = tid & 31;
-  int sum = 0, before = 0;           // places of one unit of each sequence: below 2^31
-  int64_t begin = 0;
-  for (int pass = 0;; ++pass)        // adds them up; finds the sequence that holds `begin`
+  int sum = 0, before = 0;           // tiles (places) of one unit of each sequence: below 2^31
+  int64_t begin = 0, last = 0;       // of this team's range; of the CTA's last team's
+  bool found = false;
+  for (int pass = 0; pass < 2; ++pass)      // adds them up; finds the sequence that holds `begin`
     for (int base = 0; base < p.B; base += kThreads) {
       if (pass == 0 || p.B > kThreads) {
         __syncthreads();
-        s_tiles[tid] = base + tid < p.B ? sequence(p, base + tid, pass == 0 && blockIdx.x == 0).tiles + kUnitCost : 0;
+        s_tiles[tid] = base + tid < p.B ? sequence(p, base + tid, pass == 0 && blockIdx.x == 0).tiles : 0;
         __syncthreads();
       }
-      const int4 x = reinterpret_cast<const int4*>(s_tiles)[lane];
-      const int mine = x.x + x.y + x.z + x.w;
+      int4 x = reinterpret_cast<const int4*>(s_tiles)[lane];
       if (pass == 0) {
-        sum += __reduce_add_sync(0xffffffffu, mine);
+        sum += __reduce_add_sync(0xffffffffu, x.x + x.y + x.z + x.w);
         if (base + kThreads < p.B) continue;
-        const int64_t total = (int64_t)sum * units;
-        r.n = (uint32_t)min((int64_t)gridDim.x, quotient(total + kMinTiles - 1, kMinTiles));
-        if (blockIdx.x >= r.n) return false;
+        team = (int64_t)p.B * units >= 2 * gridDim.x && sum <= (int64_t)kShort * p.B ? 1 : kWarps;
+        w.cost = unit_cost(team);
+        const int64_t total = ((int64_t)sum + (int64_t)w.cost * p.B) * units;
+        const uint32_t teams = gridDim.x * (kWarps / team), least = least_places(team);
+        r.n = (uint32_t)min((int64_t)teams, quotient(total + least - 1, least));
+        const uint32_t first = blockIdx.x * (kWarps / team), mine = first + (team == 1 ? tid / 32 : 0);
+        if (first >= r.n) return false;
         r.each = quotient(total, r.n);
         r.over = (uint32_t)(total - r.each * r.n);
-        begin = r.begin(blockIdx.x);
-        w.left = r.begin(blockIdx.x + 1) - begin;
+        last = r.begin(min(first + kWarps / team, r.n) - 1);
+        begin = r.begin(min(mine, r.n));
+        w.left = mine < r.n ? r.begin(mine + 1) - begin : 0;
         continue;
       }
+      if (x.x > 0) x.x += w.cost;    // a sequence has a tile at least
+      if (x.y > 0) x.y += w.cost;
+      if (x.z > 0) x.z += w.cost;
+      if (x.w > 0) x.w += w.cost;
+      const int mine = x.x + x.y + x.z + x.w;
       int incl = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -178,23 +194,26 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_
         if (lane >= o) incl += up;
       }
       const uint32_t here = __ballot_sync(0xffffffffu, begin < (int64_t)(before + incl) * units);
+      if (here != 0 && !found) {
+        const int from = __ffs(here) - 1;
+        int first = before + incl - mine, k = 0;      // of the lane's four sequences
+        if (begin >= (int64_t)(first + x.x) * units) { first += x.x; k = 1;
+          if (begin >= (int64_t)(first + x.y) * units) { first += x.y; k = 2;
+            if (begin >= (int64_t)(first + x.z) * units) { first += x.z; k = 3; } } }
+        first = __shfl_sync(0xffffffffu, first, from);
+        w.b = __shfl_sync(0xffffffffu, base + lane * 4 + k, from);
+        w.s = sequence(p, w.b);
+        const int64_t off = begin - (int64_t)first * units;
+        w.unit = (int)quotient(off, (uint32_t)w.places());
+        const int place = (int)(off - (int64_t)w.unit * w.places());
+        at = begin - place;
+        w.enter(place);
+        found = w.t1 > w.t0;
+      }
       before += __shfl_sync(0xffffffffu, incl, 31);
-      if (here == 0) continue;
-      const int from = __ffs(here) - 1;
-      int first = before - __shfl_sync(0xffffffffu, incl, 31) + incl - mine, k = 0;      // of the lane's four sequences
-      if (begin >= (int64_t)(first + x.x) * units) { first += x.x; k = 1;
-        if (begin >= (int64_t)(first + x.y) * units) { first += x.y; k = 2;
-          if (begin >= (int64_t)(first + x.z) * units) { first += x.z; k = 3; } } }
-      first = __shfl_sync(0xffffffffu, first, from);
-      w.b = __shfl_sync(0xffffffffu, base + lane * 4 + k, from);
-      w.s = sequence(p, w.b);
-      const int64_t off = begin - (int64_t)first * units;
-      w.unit = (int)quotient(off, (uint32_t)w.places());
-      const int place = (int)(off - (int64_t)w.unit * w.places());
-      at = begin - place;
-      w.enter(place);
-      return w.t1 > w.t0;
+      if (last < (int64_t)before * units) return found;      // the same for all warps, which meet above
     }
+  return found;
 }
 // The same where a cluster of C CTAs has a unit: an even share of its tiles (none for some where there are few).
 __device__ __forceinline__ void locate_cluster(const DecodeParams& p, int units, Walk& w) {
@@ -205,6 +224,7 @@ __device__ __forceinline__ void locate_cluster(const DecodeParams& p, int units,
   w.t0 = (int)((uint32_t)w.s.tiles * rank / p.cluster);           // tiles below 2^27, rank below 16
   w.t1 = (int)((uint32_t)w.s.tiles * (rank + 1) / p.cluster);
   w.left = 0;
+  w.cost = 0;
 }
 
 // The new token's own row of head h: turned, written to its place in the cache (page, slot) and to the copies, and the key to its
@@ -298,7 +318,8 @@ template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to,
 template <typename T, int D> struct Loader {
   Walk w;
   int tile;                          // this warp's next one, of w
-  int base, page0, page1;            // pages of the first and the last key of this lane's tile, base + kWarps lane, fetched ahead for 32 of them
+  int team, rank;                    // the team's size, this warp's place in it
+  int base, page0, page1;            // pages of the first and the last key of this lane's tile, base + team lane, fetched ahead for 32 of them
   bool more;
   uint32_t ring;
   int stage;
@@ -306,47 +327,47 @@ template <typename T, int D> struct Loader {
 
   static constexpr int kChunks = D / 8;
 
-  __device__ __forceinline__ void settle(const DecodeParams& p, int units, int warp, bool fetch) {      // at a tile of this warp, or at the end
+  __device__ __forceinline__ void settle(const DecodeParams& p, int units, bool fetch) {      // at a tile of this warp, or at the end
     while (more && tile >= w.t1) {
       more = w.next(p, units);
-      tile = w.t0 + warp;
+      tile = w.t0 + rank;
       fetch = true;
     }
-    if (!(fetch || tile == base + 32 * kWarps)) return;
+    if (!(fetch || tile == base + 32 * team)) return;
     base = tile;
     page0 = page1 = -1;
-    const int mine = tile + kWarps * (int)(threadIdx.x & 31);
+    const int mine = tile + team * (int)(threadIdx.x & 31);
     if (!more || mine >= w.t1 || mine * kTile >= w.s.len) return;
     const int first = mine * kTile;
     const int* row = p.pages.table + w.b * p.pages.table_stride;
     page0 = __ldg(row + p.pages.by_page.div((uint32_t)first));
     page1 = __ldg(row + p.pages.by_page.div((uint32_t)min(first + kTile, w.s.len) - 1u));
   }
-  __device__ __forceinline__ void start(const DecodeParams& p, int units, int warp, const Walk& from, uint32_t ring_) {
-    w = from; more = true; tile = w.t0 + warp; stage = 0; ring = ring_;
+  __device__ __forceinline__ void start(const DecodeParams& p, int units, int team_, int rank_, const Walk& from, uint32_t ring_) {
+    w = from; more = true; team = team_; rank = rank_; tile = w.t0 + rank; stage = 0; ring = ring_;
     const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
     to_k = r * D * 2 + (c ^ k_swizzle(r)) * 16;
     to_v = kTile * D * 2 + r * D * 2 + (c ^ r) * 16;
-    settle(p, units, warp, true);
+    settle(p, units, true);
   }
   // Issues the copies of one tile (none at the end); `masks` in shared memory get a bit for each key that is there.
-  __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, int warp, uint32_t* masks) {
+  __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, uint32_t* masks) {
     if (more) {
       const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
       const int first = tile * kTile, h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
       const uint32_t slot = ring + stage * stage_bytes<D>();
       const int row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
-      const int page = __shfl_sync(0xffffffffu, page0, (tile - base) / kWarps);
+      const int page = __shfl_sync(0xffffffffu, page0, team == 1 ? tile - base : (tile - base) / kWarps);
       if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page >= 0 && page < p.pages.num_pages) {
         // sixteen rows of one page
         if (lane == 0) masks[stage] = 0xffffu;
         copy_rows<D, false>(slot + to_k, rotary::chunk_at(p.pages.k, p.pages.k.off(page, row0 + r, h), c), p.pages.k.st);
         copy_rows<D, true>(slot + to_v, rotary::chunk_at(p.pages.v, p.pages.v.off(page, row0 + r, h), c), p.pages.v.st);
       } else {
-        mixed_tile<T, D>(p, w, h, w.unit == h * query_blocks, first, page, __shfl_sync(0xffffffffu, page1, (tile - base) / kWarps), slot, masks + stage);
+        mixed_tile<T, D>(p, w, h, w.unit == h * query_blocks, first, page, __shfl_sync(0xffffffffu, page1, team == 1 ? tile - base : (tile - base) / kWarps), slot, masks + stage);
       }
-      tile += kWarps;
-      settle(p, units, warp, false);
+      tile += team;
+      settle(p, units, false);
     }
     copies_commit();
     stage = stage + 1 == stages<D>() ? 0 : stage + 1;
@@ -405,23 +426,31 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   Range range{};
   Walk w;
   int64_t at = 0;                            // the place of the walk's unit in the row of all units
+  int team = kWarps;
   if (p.cluster != 0) {
     locate_cluster(p, units, w);
-  } else if (!locate(p, units, reinterpret_cast<int*>(s_acc), range, w, at)) {
-    if (tid == 0) p.parts[blockIdx.x] = make_int2(0, 0);
-    return;
+  } else {
+    const bool work = locate(p, units, reinterpret_cast<int*>(s_acc), team, range, w, at);
+    if (!work) {
+      if (lane == 0 && (team == 1 || warp == 0)) p.parts[warp * gridDim.x + blockIdx.x] = make_int2(0, team == 1 ? -1 : 0);
+      return;
+    }
   }
+  const int rank = team == 1 ? 0 : warp;
+  const uint32_t worker = team == 1 ? blockIdx.x * kWarps + warp : blockIdx.x;
   Loader<T, D> loader;
-  loader.start(p, units, warp, w, ring);
+  loader.start(p, units, team, rank, w, ring);
 
   // places of this lane's chunks in a stage: K of row g (even and odd j), V of row lane % 16, chunk lane / 16
   const uint32_t k_even = g * D * 2 + (t ^ k_swizzle(g)) * 16, k_odd = g * D * 2 + ((4 + t) ^ k_swizzle(g)) * 16;
   const uint32_t v_place = (kTile + lane % 16) * D * 2 + ((lane >> 4) ^ (lane & 7)) * 16;
   int stage = 0, turned_b = -1, tile = 0, h = 0, q0 = 0;
-  int2 part = make_int2(0, 0);
+  int2 part = make_int2(0, team == 1 ? -1 : 0);
   uint32_t qh[D / 32][4], ql[D / 32][4];     // this lane's part of the queries, in two 16-bit halves
   float m = 0.f, l = 0.f, acc[D / 8][4];
-  const double inv_freq = p.rot.inv_freq != nullptr && tid < p.rot.rot / 2 ? p.rot.inv_freq[tid] : 0.;
+  float2* cs = team == 1 ? reinterpret_cast<float2*>(s_acc) + (1 + warp) * 64 : s_cs;      // behind what locate() may still be reading
+  const int cs_first = team == 1 ? lane : tid;
+  const double inv_freq = p.rot.inv_freq != nullptr && cs_first < p.rot.rot / 2 ? p.rot.inv_freq[cs_first] : 0.;
   // What a unit begins with: its queries' rows, and cosines and sines of their position, one a thread (those of the unit before have been
   // read: its parts have been joined).
   auto fetch = [&]() {
@@ -434,7 +463,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 #pragma unroll
       for (int e = 0; e < 4; ++e) qh[j][e] = (&x.x)[e];
     }
-    if (tid < p.rot.rot / 2 && turned_b != w.b) s_cs[tid] = rotary::cos_sin(p.rot, inv_freq, p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
+    if (turned_b != w.b)
+      for (int i = cs_first; i < p.rot.rot / 2; i += 32 * team)
+        cs[i] = rotary::cos_sin(p.rot, i == cs_first ? inv_freq : p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
     turned_b = w.b;
   };
   // Steps 1 - kStages to -1 only copy.  A step's copies are issued between the scores' products and what waits for them, and at
@@ -451,54 +482,72 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           // the warps' parts
           l += __shfl_xor_sync(0xffffffffu, l, 1);
           l += __shfl_xor_sync(0xffffffffu, l, 2);
-          __syncthreads();                         // the part before has been read
-          if (t == 0) s_ml[warp][g] = make_float2(m, l);
-          if (row_there) {
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
-              float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
-              *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
-            }
-          }
-          __syncthreads();
           const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
           const bool whole = p.cluster != 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
-          constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
-          const int r = tid / 16, d0 = (tid % 16) * kEach;
-          if (q0 + r < p.G) {
-            float top = -INFINITY;
+          if (team == 1) {
+            if (row_there) {
+              const float inv = l == 0.f ? 0.f : 1.f / l;
+              const int64_t at_row = ((int64_t)worker * 2 + (from_start ? 1 : 0)) * kQ + g;
+              uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + g, h) + 2 * t));
 #pragma unroll
-            for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i][r].x);
-            const float base = top == -INFINITY ? 0.f : top;
-            float sum = 0.f, out[kEach] = {};
-#pragma unroll
-            for (int i = 0; i < kWarps; ++i) {
-              const float weight = fast_exp2(s_ml[i][r].x - base);
-              sum = fmaf(s_ml[i][r].y, weight, sum);
-#pragma unroll
-              for (int e = 0; e < kEach; e += 4) {
-                const float4 x = *part_at<D>(s_acc, i, r, (d0 + e) / 4);
-                out[e] = fmaf(x.x, weight, out[e]);
-                out[e + 1] = fmaf(x.y, weight, out[e + 1]);
-                out[e + 2] = fmaf(x.z, weight, out[e + 2]);
-                out[e + 3] = fmaf(x.w, weight, out[e + 3]);
+              for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
+                const float x = acc[n][0] + acc[n][2], y = acc[n][1] + acc[n][3];
+                if (whole) to[4 * n] = Pack<T>::pack(x * inv, y * inv);
+                else *reinterpret_cast<float2*>(p.acc + at_row * D + 8 * n + 2 * t) = make_float2(x, y);
+              }
+              if (t == 0) {
+                if (whole) p.lse[((int64_t)w.b * p.G + q0 + g) * p.H + h] = m + log2f(l);
+                else p.ml[at_row] = make_float2(m, l);
               }
             }
-            if (whole) {
-              const float inv = sum == 0.f ? 0.f : 1.f / sum;
-              uint32_t packed[kEach / 2];
+          } else {
+            __syncthreads();                         // the part before has been read
+            if (t == 0) s_ml[warp][g] = make_float2(m, l);
+            if (row_there) {
 #pragma unroll
-              for (int e = 0; e < kEach / 2; ++e) packed[e] = Pack<T>::pack(out[2 * e] * inv, out[2 * e + 1] * inv);
-              uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d0));
+              for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
+                float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
+                *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+              }
+            }
+            __syncthreads();
+            constexpr int kEach = D / 16;            // elements of a thread: 16 threads a row
+            const int r = tid / 16, d0 = (tid % 16) * kEach;
+            if (q0 + r < p.G) {
+              float top = -INFINITY;
 #pragma unroll
-              for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
-              if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
-            } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
-              const int64_t at_row = p.cluster != 0 ? r : ((int64_t)blockIdx.x * 2 + (from_start ? 1 : 0)) * kQ + r;
-              float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
+              for (int i = 0; i < kWarps; ++i) top = fmaxf(top, s_ml[i][r].x);
+              const float base = top == -INFINITY ? 0.f : top;
+              float sum = 0.f, out[kEach] = {};
 #pragma unroll
-              for (int e = 0; e < kEach; ++e) to[e] = out[e];
-              if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
+              for (int i = 0; i < kWarps; ++i) {
+                const float weight = fast_exp2(s_ml[i][r].x - base);
+                sum = fmaf(s_ml[i][r].y, weight, sum);
+#pragma unroll
+                for (int e = 0; e < kEach; e += 4) {
+                  const float4 x = *part_at<D>(s_acc, i, r, (d0 + e) / 4);
+                  out[e] = fmaf(x.x, weight, out[e]);
+                  out[e + 1] = fmaf(x.y, weight, out[e + 1]);
+                  out[e + 2] = fmaf(x.z, weight, out[e + 2]);
+                  out[e + 3] = fmaf(x.w, weight, out[e + 3]);
+                }
+              }
+              if (whole) {
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                uint32_t packed[kEach / 2];
+#pragma unroll
+                for (int e = 0; e < kEach / 2; ++e) packed[e] = Pack<T>::pack(out[2 * e] * inv, out[2 * e + 1] * inv);
+                uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d0));
+#pragma unroll
+                for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
+                if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
+              } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
+                const int64_t at_row = p.cluster != 0 ? r : ((int64_t)worker * 2 + (from_start ? 1 : 0)) * kQ + r;
+                float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) to[e] = out[e];
+                if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
+              }
             }
           }
           if (p.cluster != 0) {
@@ -508,19 +557,20 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
             const int64_t last = at + w.places() - 1;
             uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
-            while (range.begin(blockIdx.x + n) > last) --n;
-            while (range.begin(blockIdx.x + n + 1) <= last) ++n;
-            part = make_int2(w.b * units + w.unit, (int)n + 1);
+            while (range.begin(worker + n) > last) --n;
+            while (range.begin(worker + n + 1) <= last) ++n;
+            part = make_int2(w.b * units + w.unit, ((int)n + 1) * (team == 1 ? -1 : 1));
           }
           at += w.places();
           if (!w.next(p, units)) {
-            if (tid == 0) p.parts[blockIdx.x] = part;
+            if (lane == 0 && rank == 0) p.parts[(team == 1 ? warp * gridDim.x : 0) + blockIdx.x] = part;
             return;
           }
           fetch();
         }
         const bool row_there = q0 + g < p.G;
-        if (p.rot.inv_freq != nullptr) __syncthreads();
+        if (team == 1) __syncwarp();
+        else if (p.rot.inv_freq != nullptr) __syncthreads();
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const int chunk = 4 * j + t;
@@ -532,9 +582,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
             if (p.rot.interleaved) {
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const float2 a = Pack<T>::unpack(qh[j][e]), cs = s_cs[chunk * 4 + e];
-                y[2 * e] = fmaf(a.x, cs.x, -a.y * cs.y);
-                y[2 * e + 1] = fmaf(a.y, cs.x, a.x * cs.y);
+                const float2 a = Pack<T>::unpack(qh[j][e]), turn = cs[chunk * 4 + e];
+                y[2 * e] = fmaf(a.x, turn.x, -a.y * turn.y);
+                y[2 * e + 1] = fmaf(a.y, turn.x, a.x * turn.y);
               }
             } else {
               const int half = p.rot.rot >> 4;                     // chunks
@@ -544,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float2 a = Pack<T>::unpack(qh[j][e]), b = Pack<T>::unpack((&other.x)[e]);
-                const float2 c0 = s_cs[pair + 2 * e], c1 = s_cs[pair + 2 * e + 1];
+                const float2 c0 = cs[pair + 2 * e], c1 = cs[pair + 2 * e + 1];
                 y[2 * e] = fmaf(a.x, c0.x, second ? b.x * c0.y : -b.x * c0.y);
                 y[2 * e + 1] = fmaf(a.y, c1.x, second ? b.y * c1.y : -b.y * c1.y);
               }
@@ -556,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         m = -INFINITY; l = 0.f;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-        tile = w.t0 + warp;
+        tile = w.t0 + rank;
         begins = false;
       }
       copies_wait<kStages - 2>();
@@ -574,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         }
       }
     }
-    loader.issue(p, units, query_blocks, warp, s_masks[warp]);
+    loader.issue(p, units, query_blocks, s_masks[warp]);
     if (step < 0) continue;
     float x[4];                            // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
@@ -613,68 +663,75 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       mma<T>(acc[2 * j + 1], ph[0], pl[0], ph[1], pl[1], v[2], v[3]);
     }
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    tile += kWarps;
+    tile += team;
   }
 }
 // Joins the parts of the units that several CTAs hold.  Grid: (CTA in which the unit begins, query row).  A warp takes every eighth
 // part, five of them on the way together: 40 parts, what one sequence with 8 heads has, take one trip to memory.
 constexpr int kJoinWarps = 8, kJoinAhead = 5;
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) join_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 5) join_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float s_acc[kJoinWarps][D];
   __shared__ float2 s_ml[kJoinWarps];
   grid_before();
-  const int2 part = p.parts[blockIdx.x];
-  const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
-  const int r = blockIdx.y, b = part.x / units, u = part.x - b * units, h = u / query_blocks, row = (u - h * query_blocks) * kQ + r;
-  if (part.y < 2 || row >= p.G) return;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  auto place = [&](int i) { return ((int64_t)(blockIdx.x + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
-  constexpr int kEach = D / 32;
-  float top = -INFINITY, sum = 0.f, out[kEach] = {};
-  for (int i0 = warp; i0 < part.y; i0 += kJoinAhead * kJoinWarps) {
-    float2 ml[kJoinAhead];
-    float x[kJoinAhead][kEach];
+  int2 part = p.parts[blockIdx.x];
+  if (part.y == 0) return;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, r = blockIdx.y;
+  const bool by_warps = part.y < 0;          // four teams' parts; or the CTA's
+#pragma unroll 1
+  for (int k = 0; k < (by_warps ? kWarps : 1); ++k) {
+    if (k > 0) part = p.parts[k * gridDim.x + blockIdx.x];
+    const int id = part.x, n = abs(part.y);
+    if (n < 2) continue;                     // the same for all threads, as is what follows
+    const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
+    const int b = id / units, u = id - b * units, h = u / query_blocks, row = (u - h * query_blocks) * kQ + r;
+    if (row >= p.G) continue;
+    const int64_t first = by_warps ? blockIdx.x * kWarps + k : blockIdx.x;      // the team
+    auto place = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
+    constexpr int kEach = D / 32;
+    float top = -INFINITY, sum = 0.f, out[kEach] = {};
+    for (int i0 = warp; i0 < n; i0 += kJoinAhead * kJoinWarps) {
+      float2 ml[kJoinAhead];
+      float x[kJoinAhead][kEach];
 #pragma unroll
-    for (int k = 0; k < kJoinAhead; ++k) {
-      const int64_t at = place(min(i0 + k * kJoinWarps, part.y - 1));      // beyond the last one: it again, unused
-      ml[k] = p.ml[at];
-      const float* from = p.acc + at * D + lane * kEach;
-      if constexpr (kEach == 4) *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(from);
-      else *reinterpret_cast<float2*>(x[k]) = *reinterpret_cast<const float2*>(from);
+      for (int i = 0; i < kJoinAhead; ++i) {
+        const int64_t at = place(min(i0 + i * kJoinWarps, n - 1));      // beyond the last one: it again, unused
+        ml[i] = p.ml[at];
+        const float* from = p.acc + at * D + lane * kEach;
+        if constexpr (kEach == 4) *reinterpret_cast<float4*>(x[i]) = *reinterpret_cast<const float4*>(from);
+        else *reinterpret_cast<float2*>(x[i]) = *reinterpret_cast<const float2*>(from);
+      }
+#pragma unroll
+      for (int i = 0; i < kJoinAhead; ++i) {
+        if (i0 + i * kJoinWarps >= n) break;
+        const float now = fmaxf(top, ml[i].x), base = now == -INFINITY ? 0.f : now, was = fast_exp2(top - base), is = fast_exp2(ml[i].x - base);
+        sum = sum * was + ml[i].y * is;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) out[e] = out[e] * was + x[i][e] * is;
+        top = now;
+      }
     }
+    __syncthreads();                         // the unit before has been read
 #pragma unroll
-    for (int k = 0; k < kJoinAhead; ++k) {
-      if (i0 + k * kJoinWarps >= part.y) break;
-      const float now = fmaxf(top, ml[k].x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(ml[k].x - base);
-      sum = sum * a + ml[k].y * b;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) out[e] = out[e] * a + x[k][e] * b;
-      top = now;
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) s_acc[warp][lane * kEach + e] = out[e];
-  if (lane == 0) s_ml[warp] = make_float2(top, sum);
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, s_ml[i].x);
-  const float base = top == -INFINITY ? 0.f : top;
-  float weight[kJoinWarps];
-  sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) {
-    weight[i] = fast_exp2(s_ml[i].x - base);
-    sum = fmaf(s_ml[i].y, weight[i], sum);
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = threadIdx.x; d < D / 2; d += kJoinWarps * 32) {
+    for (int e = 0; e < kEach; ++e) s_acc[warp][lane * kEach + e] = out[e];
+    if (lane == 0) s_ml[warp] = make_float2(top, sum);
+    __syncthreads();
+    if (threadIdx.x >= D / 2) continue;      // two elements a thread
+    const int held_by = min(n, kJoinWarps), d = threadIdx.x;
+    for (int i = 0; i < held_by; ++i) top = fmaxf(top, s_ml[i].x);
+    const float base = top == -INFINITY ? 0.f : top;
     float x = 0.f, y = 0.f;
-#pragma unroll
-    for (int i = 0; i < kJoinWarps; ++i) { x = fmaf(s_acc[i][2 * d], weight[i], x); y = fmaf(s_acc[i][2 * d + 1], weight[i], y); }
+    sum = 0.f;
+    for (int i = 0; i < held_by; ++i) {
+      const float weight = fast_exp2(s_ml[i].x - base);
+      sum = fmaf(s_ml[i].y, weight, sum);
+      x = fmaf(s_acc[i][2 * d], weight, x);
+      y = fmaf(s_acc[i][2 * d + 1], weight, y);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * p.o.off(b, row, h))[d] = Pack<T>::pack(x * inv, y * inv);
+    if (d == 0) p.lse[((int64_t)b * p.G + row) * p.H + h] = top + log2f(sum);
   }
-  if (threadIdx.x == 0) p.lse[((int64_t)b * p.G + row) * p.H + h] = top + log2f(sum);
 }
 
 }  // namespace paged

@@ -116,12 +116,13 @@ Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
   int cluster = 1;
   while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
   if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
-  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, (units * (tiles + paged::kUnitCost) + paged::kMinTiles - 1) / paged::kMinTiles)), 0};
+  const int cost = paged::unit_cost(paged::kWarps), least = paged::least_places(paged::kWarps);
+  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, (units * (tiles + cost) + least - 1) / least)), 0};
 }
 // Scratch of an evenly divided call: which units are shared, their parts' maxima and sums, their parts.
-size_t parts_bytes(int n) { return ((size_t)n * sizeof(int2) + 255) & ~(size_t)255; }
-size_t ml_bytes(int n) { return (size_t)n * 2 * paged::kQ * sizeof(float2); }
-size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * 2 * paged::kQ * D * sizeof(float); }
+size_t parts_bytes(int n) { return ((size_t)n * paged::kWarps * sizeof(int2) + 255) & ~(size_t)255; }
+size_t ml_bytes(int n) { return (size_t)n * paged::kWarps * 2 * paged::kQ * sizeof(float2); }
+size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * paged::kWarps * 2 * paged::kQ * D * sizeof(float); }
 
 template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, int device, cudaStream_t st) {
   auto kern = paged::decode_kernel<T, D>;
@@ -275,7 +276,7 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   }
   // the kernels count keys, and the tiles of one head of all sequences, in 31 bits
   const int64_t most_keys = (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L;
-  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 1 + paged::kUnitCost) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
+  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 1 + paged::unit_cost(paged::kWarps)) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
   const int n_sm = sm_count(prob->device);
