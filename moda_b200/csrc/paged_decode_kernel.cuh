@@ -100,9 +100,12 @@ __device__ __forceinline__ void load_transposed(uint32_t (&x)[4], uint32_t at) {
 
 template <int D> __host__ __device__ constexpr int stage_bytes() { return kTile * D * 2 * 2; }
 __host__ __device__ constexpr int k_swizzle(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
-template <int D> __host__ __device__ constexpr int stages() { return D == 128 ? 3 : 6; }      // 24 KB a warp
-// The copies' slots and the warps' parts of a unit.  With what the kernel declares statically, two CTAs just fit an SM.
-template <int D> constexpr size_t smem_bytes() { return (size_t)kWarps * stages<D>() * stage_bytes<D>() + (size_t)kWarps * kQ * D * 4; }
+constexpr int kStages = 3;
+// Rows of 64 elements take half the products and half the registers for them, and nearly as many other instructions a tile: three CTAs an
+// SM.  213 sequences of up to 986 rows, 10 heads of 64: 82 us with two (and six stages), 73 with three, 123 with four, whose registers spill.
+template <int D> __host__ __device__ constexpr int ctas_per_sm() { return D == 128 ? 2 : 3; }
+// The copies' slots and the warps' parts of a unit.  With what the kernel declares statically, two CTAs just fit an SM (D = 128).
+template <int D> constexpr size_t smem_bytes() { return (size_t)kWarps * kStages * stage_bytes<D>() + (size_t)kWarps * kQ * D * 4; }
 // Four elements from 4 chunk on of a row of those parts; the order of a row's chunks spreads the lanes over the banks.
 template <int D> __device__ __forceinline__ float4* part_at(float* parts, int warp, int row, int chunk) {
   return reinterpret_cast<float4*>(parts + (warp * kQ + row) * D) + (chunk ^ row);
@@ -370,7 +373,7 @@ template <typename T, int D> struct Loader {
       settle(p, units, false);
     }
     copies_commit();
-    stage = stage + 1 == stages<D>() ? 0 : stage + 1;
+    stage = stage + 1 == kStages ? 0 : stage + 1;
   }
 };
 
@@ -409,13 +412,12 @@ __device__ __forceinline__ void join_cluster(const DecodeParams& p, const Walk& 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ uint32_t s_masks[kWarps][stages<D>()];
+  __shared__ uint32_t s_masks[kWarps][kStages];
   __shared__ float2 s_ml[kWarps][kQ];
   __shared__ float2 s_cs[D / 2];
   __shared__ float2 s_part_ml[kQ];
-  constexpr int kStages = stages<D>();
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
   const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
   const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();

@@ -100,18 +100,20 @@ template <typename T> __device__ __forceinline__ void turn(uint4& x, uint4& y, c
   }
 }
 
-// The eight cosines and sines of this lane's item at position pos.  The 32 / C lanes of an item compute 8 C / 32 each.
-template <int C> __device__ __forceinline__ void item_cos_sin(const Args& a, int lane, long long pos, float2 (&cs)[8]) {
-  constexpr int kEach = 8 * C / 32;
-  const int c = lane % C, v = lane / C;
+// The eight cosines and sines of this lane's item at its token's position pos.  Of the warp's 32 lanes, 32 / (C kTokens) have the same item
+// and token and compute an equal share each.
+template <int C, int kTokens = 1> __device__ __forceinline__ void item_cos_sin(const Args& a, int lane, long long pos, float2 (&cs)[8]) {
+  constexpr int kShare = 32 / (C * kTokens), kEach = 8 / kShare;
+  const int c = lane % C, v = lane / C % kShare;
   float2 mine[kEach];
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
     mine[i] = c < (a.rot >> 4) ? cos_sin(a, a.inv_freq[8 * c + v * kEach + i], pos) : make_float2(1.f, 0.f);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    cs[i].x = __shfl_sync(0xffffffffu, mine[i % kEach].x, (i / kEach) * C + c);
-    cs[i].y = __shfl_sync(0xffffffffu, mine[i % kEach].y, (i / kEach) * C + c);
+    const int from = lane + (i / kEach - v) * C;
+    cs[i].x = __shfl_sync(0xffffffffu, mine[i % kEach].x, from);
+    cs[i].y = __shfl_sync(0xffffffffu, mine[i % kEach].y, from);
   }
 }
 
@@ -143,29 +145,29 @@ struct RotaryParams {
 constexpr int kThreads = 128, kBlocks = 8;      // an SM: 32 warps, 64 registers a thread
 constexpr int kBatch = 2;    // vectors whose loads a lane has under way together
 
-// Grid: x over the tokens (a warp each), y over shares of a token's vectors.
-template <typename T, int D>
+// Grid: x over the tokens (kTokens a warp), y over shares of a token's vectors.
+template <typename T, int D, int kTokens>
 __global__ void __launch_bounds__(kThreads, kBlocks) rotary_kernel(const __grid_constant__ RotaryParams p) {
   grid_before();
-  constexpr int C = D / 16, kLanes = 32 / C;
+  constexpr int C = D / 16, kLanes = 32 / (C * kTokens);      // kLanes vectors of a token at a time
   const int lane = threadIdx.x % 32, c = lane % C;
-  const int64_t tokens = (int64_t)p.B * p.T;
   const int first = blockIdx.y * p.per_warp, last = min(first + p.per_warp, p.vectors);
   int c0, c1;
   const bool turns = item_chunks(p.rot, c, c0, c1);
   const bool interleaved = p.rot.interleaved != 0;
-  const int64_t tok = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  if (tok >= tokens) return;
-  const int b = (int)p.by_t.div((uint32_t)tok), t = (int)(tok - (int64_t)b * p.T);
+  const int64_t tok = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kTokens + lane / (C * kLanes);
+  const bool active = tok < (int64_t)p.B * p.T;
+  const int b = active ? (int)p.by_t.div((uint32_t)tok) : 0, t = active ? (int)(tok - (int64_t)b * p.T) : 0;
   float2 cs[8];
-  for (int v0 = first + lane / C, step = 0; first + step * kBatch * kLanes < last; v0 += kBatch * kLanes, ++step) {      // uniform over the warp
+  for (int step = 0; first + step * kBatch * kLanes < last; ++step) {      // uniform over the warp
+    const int v0 = first + step * kBatch * kLanes + lane / C % kLanes;
     uint4 x[kBatch], y[kBatch];
     int64_t out[kBatch];
     bool is_k[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int v = v0 + i * kLanes;
-      if (v >= last) continue;
+      if (v >= last || !active) continue;
       const int g = (int)p.by_h.div((uint32_t)v), h = v - g * p.H;
       is_k[i] = g == p.G;
       const View& in = is_k[i] ? p.k : p.q;
@@ -174,10 +176,10 @@ __global__ void __launch_bounds__(kThreads, kBlocks) rotary_kernel(const __grid_
       x[i] = *chunk_at(in, off, c0);
       y[i] = *chunk_at(in, off, c1);
     }
-    if (step == 0) item_cos_sin<C>(p.rot, lane, p.pos.at(b, t), cs);      // while they are on the way
+    if (step == 0) item_cos_sin<C, kTokens>(p.rot, lane, p.pos.at(b, t), cs);      // while they are on the way
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (v0 + i * kLanes >= last) continue;
+      if (v0 + i * kLanes >= last || !active) continue;
       if (turns) turn<T>(x[i], y[i], cs, interleaved);
       const View& to = is_k[i] ? p.k_out : p.q_out;
       *chunk_at(to, out[i], c0) = x[i];
@@ -220,53 +222,56 @@ struct AppendParams {
   FastDiv by_t;
 };
 
-template <typename T, int D>
+template <typename T, int D, int kTokens>
 __global__ void __launch_bounds__(rotary::kThreads, rotary::kBlocks) append_kernel(const __grid_constant__ AppendParams p) {
   using namespace rotary;
   grid_before();
-  constexpr int C = D / 16, kLanes = 32 / C;
+  constexpr int C = D / 16, kLanes = 32 / (C * kTokens);
   const int lane = threadIdx.x % 32, c = lane % C;
-  const int64_t tokens = (int64_t)p.B * p.T;
   const int first = blockIdx.y * p.per_warp, last = min(first + p.per_warp, 2 * p.H);
   int c0, c1;
   const bool turns = item_chunks(p.rot, c, c0, c1) && p.rot.inv_freq != nullptr;
   const bool interleaved = p.rot.interleaved != 0;
-  const int64_t tok = (int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  if (tok >= tokens) return;
-  const int b = (int)p.by_t.div((uint32_t)tok), t = (int)(tok - (int64_t)b * p.T);
-  if (p.lengths != nullptr && t >= p.lengths[b]) return;
+  const int64_t tok = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kTokens + lane / (C * kLanes);
+  bool active = tok < (int64_t)p.B * p.T;
+  const int b = active ? (int)p.by_t.div((uint32_t)tok) : 0, t = active ? (int)(tok - (int64_t)b * p.T) : 0;
+  active = active && (p.lengths == nullptr || t < p.lengths[b]);
+  if (!__any_sync(0xffffffffu, active)) return;
   float2 cs[8];
   int page = 0, slot = 0;
-  for (int v0 = first + lane / C, step = 0; first + step * kBatch * kLanes < last; v0 += kBatch * kLanes, ++step) {      // uniform over the warp
+  for (int step = 0; first + step * kBatch * kLanes < last; ++step) {      // uniform over the warp
+    const int v0 = first + step * kBatch * kLanes + lane / C % kLanes;
     uint4 x[kBatch], y[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int v = v0 + i * kLanes;
-      if (v >= last) continue;
+      if (v >= last || !active) continue;
       const View& in = v < p.H ? p.k : p.v;
       const int64_t off = in.off(b, t, v < p.H ? v : v - p.H);
       x[i] = *chunk_at(in, off, c0);
       y[i] = *chunk_at(in, off, c1);
     }
-    if (step == 0) {                       // the place and the angles, while the rows are on the way
+    if (step == 0) {                         // the place and the angles, while the rows are on the way
       const int64_t n = (int64_t)p.pages.seq_lens[b] + t;
-      if (n < 0 || n >= p.pages.room) {
-        if (lane == 0) wrong(kBadLength);
-        return;
+      if (active && (n < 0 || n >= p.pages.room)) {
+        active = false;
+        wrong(kBadLength);
       }
-      const int which = (int)p.pages.by_page.div((uint32_t)n);
-      page = p.pages.table[b * p.pages.table_stride + which];
-      slot = (int)n - which * p.pages.page_size;
-      if (p.rot.inv_freq != nullptr && first < p.H) item_cos_sin<C>(p.rot, lane, n, cs);
-      if (page < 0 || page >= p.pages.num_pages) {
-        if (lane == 0) wrong(kBadPage);
-        return;
+      if (active) {
+        const int which = (int)p.pages.by_page.div((uint32_t)n);
+        page = p.pages.table[b * p.pages.table_stride + which];
+        slot = (int)n - which * p.pages.page_size;
+      }
+      if (p.rot.inv_freq != nullptr && first < p.H) item_cos_sin<C, kTokens>(p.rot, lane, n, cs);
+      if (active && (page < 0 || page >= p.pages.num_pages)) {
+        active = false;
+        wrong(kBadPage);
       }
     }
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
       const int v = v0 + i * kLanes;
-      if (v >= last) continue;
+      if (v >= last || !active) continue;
       if (turns && v < p.H) turn<T>(x[i], y[i], cs, interleaved);
       const View& to = v < p.H ? p.pages.k : p.pages.v;
       const int64_t off = to.off(page, slot, v < p.H ? v : v - p.H);

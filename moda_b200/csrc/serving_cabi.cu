@@ -51,16 +51,21 @@ int check_pages(const moda_problem* pr, const moda_paged_cache* c, paged::Pages*
   return MODA_OK;
 }
 
-// Grid of the kernels that give a token to a warp: (tokens, shares of its vectors).  A token whose vectors one warp
-// can walk in a few steps stays whole (the sines are computed once); few tokens are shared by more warps, down to one
-// step of kBatch vectors a lane, until there are some 16 warps for each SM.
-dim3 token_grid(int64_t tokens, int vectors, int D, int n_sm, int* per_warp) {
-  const int lanes = 32 / (D / 16), step = lanes * rotary::kBatch, warps = rotary::kThreads / 32;
-  const int most = (vectors + step - 1) / step;
+// How the kernels that turn a token's vectors are divided: tokens a warp, vectors of a token that a warp takes, grid (tokens, shares of a
+// token's vectors).  A warp has 32 / (D / 16) vectors of a token side by side, or where there are so few of them as many tokens.
+// A token that one warp can walk in a few steps stays whole (the sines are computed once); few tokens are shared by more warps, down to
+// one step of kBatch vectors a lane, until there are some 16 warps for each SM.
+struct TokenGrid { int tokens_a_warp, per_warp; dim3 grid; };
+TokenGrid token_grid(int64_t tokens, int vectors, int D, int n_sm) {
+  TokenGrid r{1, 0, dim3()};
+  int lanes = 32 / (D / 16);
+  while (r.tokens_a_warp < (D == 128 ? 2 : 4) && vectors * 2 <= lanes) { r.tokens_a_warp *= 2; lanes /= 2; }
+  const int step = lanes * rotary::kBatch, most = (vectors + step - 1) / step;
+  const int64_t a_block = (int64_t)(rotary::kThreads / 32) * r.tokens_a_warp;
   const int64_t shares = std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)n_sm * 16 / std::max<int64_t>(tokens, 1)));
-  const int steps = (int)((most + shares - 1) / shares);
-  *per_warp = steps * step;
-  return dim3((unsigned)((tokens + warps - 1) / warps), (unsigned)((vectors + *per_warp - 1) / *per_warp));
+  r.per_warp = (int)((most + shares - 1) / shares) * step;
+  r.grid = dim3((unsigned)((tokens + a_block - 1) / a_block), (unsigned)((vectors + r.per_warp - 1) / r.per_warp));
+  return r;
 }
 
 // A launch that may begin when the grid before it has ended but not flushed what it wrote: the kernels here wait for that themselves, before
@@ -82,11 +87,17 @@ cudaError_t launch(void (*kern)(P), dim3 grid, int threads, size_t smem, int clu
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kern, p);
 }
-template <typename T, int D> cudaError_t launch_rotary(const rotary::RotaryParams& p, dim3 grid, cudaStream_t st) {
-  return launch(rotary::rotary_kernel<T, D>, grid, rotary::kThreads, 0, 1, st, p);
+template <typename T, int D> cudaError_t launch_rotary(const rotary::RotaryParams& p, const TokenGrid& g, cudaStream_t st) {
+  auto kern = rotary::rotary_kernel<T, D, 1>;
+  if (g.tokens_a_warp == 2) kern = rotary::rotary_kernel<T, D, 2>;
+  if constexpr (D == 64) if (g.tokens_a_warp == 4) kern = rotary::rotary_kernel<T, D, 4>;
+  return launch(kern, g.grid, rotary::kThreads, 0, 1, st, p);
 }
-template <typename T, int D> cudaError_t launch_append(const paged::AppendParams& p, dim3 grid, cudaStream_t st) {
-  return launch(paged::append_kernel<T, D>, grid, rotary::kThreads, 0, 1, st, p);
+template <typename T, int D> cudaError_t launch_append(const paged::AppendParams& p, const TokenGrid& g, cudaStream_t st) {
+  auto kern = paged::append_kernel<T, D, 1>;
+  if (g.tokens_a_warp == 2) kern = paged::append_kernel<T, D, 2>;
+  if constexpr (D == 64) if (g.tokens_a_warp == 4) kern = paged::append_kernel<T, D, 4>;
+  return launch(kern, g.grid, rotary::kThreads, 0, 1, st, p);
 }
 
 int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v, const paged::Pages& pages, const int32_t* lengths,
@@ -94,7 +105,8 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
   paged::AppendParams p{};
   p.k = to_view(k); p.v = to_view(v); p.pages = pages; p.lengths = lengths; p.rot = rot;
   p.B = pr->B; p.T = pr->T_kv; p.H = pr->H; p.by_t = rotary::FastDiv((uint32_t)pr->T_kv);
-  const dim3 grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm, &p.per_warp);
+  const TokenGrid grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm);
+  p.per_warp = grid.per_warp;
   cudaError_t e;
   {
     prof::Scope ps(prof::kPagedAppend, st);
@@ -112,7 +124,7 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
 struct Division { int ctas, cluster; };
 Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
   const int64_t heads = (int64_t)pr->H * ((pr->G + paged::kQ - 1) / paged::kQ), units = pr->B * heads;
-  const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile), slots = 2 * n_sm;
+  const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile), slots = (int64_t)n_sm * (pr->D == 128 ? paged::ctas_per_sm<128>() : paged::ctas_per_sm<64>());
   int cluster = 1;
   while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
   if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
@@ -196,7 +208,8 @@ int moda_b200_rotary(const moda_problem* prob, const moda_rotary* rot, const mod
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const dim3 grid = token_grid(B * T, p.vectors, prob->D, n_sm, &p.per_warp);
+  const TokenGrid grid = token_grid(B * T, p.vectors, prob->D, n_sm);
+  p.per_warp = grid.per_warp;
   cudaError_t e;
   {
     prof::Scope ps(prof::kRotary, st);

@@ -126,6 +126,9 @@ APPEND = [  # dtype, T, held, lengths, H, D, page, heads, rot, interleaved
     (BF, 33, [1], None, 20, 64, 24, False, 0, False),
     (BF, 1500, [0, 100, 7], [1500, 1, 777], 4, 128, 64, True, 64, True),
     (HF, 2, list(range(150)), None, 1, 64, 8, True, 48, True),
+    (BF, 61, [0, 9, 64], [61, 3, 0], 1, 128, 16, True, 128, False),           # two and four tokens a warp
+    (HF, 31, [5, 1, 0, 77, 3], [31, 30, 1, 0, 17], 1, 64, 24, False, 64, True),
+    (BF, 3, [7] * 9, [1, 2, 3] * 3, 2, 64, 5, True, 32, False),
 ]
 
 
