@@ -33,7 +33,7 @@ constexpr int kTile = 16;          // keys of a warp's step
 constexpr int kQ = 8;              // query heads of a unit; more are further units
 // A team takes a unit: the four warps of a CTA, which divide its tiles; or, where there are many short units (kShort tiles on average),
 // each warp by itself, which has nothing to wait for.  1708 units of one tile, D = 128: 37 us by CTAs, 21 by warps.
-constexpr int kShort = 12;
+constexpr int kShort = 12, kWhole = 2 * kShort;
 // Tiles that a unit counts for beyond its own, where the work is divided: beginning and ending one takes a CTA about as long.  37
 // sequences of up to 1531 rows, 5 heads of 64 (units of 1 to 97 tiles): 23.2 us without, 18.0 with 4, 16.1 with 8, 16.8 with 16.
 __host__ __device__ constexpr int unit_cost(int team) { return team == 1 ? 2 : 8; }
@@ -111,15 +111,17 @@ template <int D> __device__ __forceinline__ float4* part_at(float* parts, int wa
   return reinterpret_cast<float4*>(parts + (warp * kQ + row) * D) + (chunk ^ row);
 }
 
-struct Sequence { int held, len, keys, tiles; };     // rows in the cache, with the token's own, with the depth rows; 16-key tiles (at least one)
+// Rows in the cache, those with the token's own, depth rows; 16-key tiles of the first two, and of all (at least one).  Depth rows begin a tile.
+struct Sequence { int held, len, depth, cached_tiles, tiles; };
 __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b, bool report = false) {
   Sequence s;
   const int len = p.pages.seq_lens[b], seen = p.depth_positions != nullptr ? p.depth_positions[b] : p.P, own = p.k.ptr != nullptr;
   if (report && (len < 0 || len > p.pages.room - own || seen < 0 || seen > p.P)) wrong(kBadLength);
   s.held = min(max(len, 0), p.pages.room);
   s.len = s.held + (len >= 0 && len < p.pages.room ? own : 0);
-  s.keys = s.len + min(max(seen, 0), p.P) * p.L;                  // below 2^31, as the tables are wide
-  s.tiles = max((s.keys + kTile - 1) / kTile, 1);
+  s.depth = min(max(seen, 0), p.P) * p.L;
+  s.cached_tiles = (s.len + kTile - 1) / kTile;                   // all below 2^31, as the tables are wide
+  s.tiles = max(s.cached_tiles + (s.depth + kTile - 1) / kTile, 1);
   return s;
 }
 
@@ -131,11 +133,16 @@ struct Walk {
   int t0, t1;
   int64_t left;                      // places of the range behind this unit
   __device__ __forceinline__ int places() const { return s.tiles + cost; }
+  // The part of the unit from `place` on.  Short units of single warps stay whole, with the team that has their first place.
   __device__ __forceinline__ void enter(int place) {
     const int used = (int)min((int64_t)(places() - place), left);
     left -= used;
     t0 = max(place - cost, 0);
     t1 = max(place + used - cost, 0);
+    if (cost == unit_cost(1) && s.tiles <= kWhole) {
+      t0 = 0;
+      t1 = place == 0 ? s.tiles : 0;
+    }
   }
   __device__ __forceinline__ bool next(const DecodeParams& p, int units) {
     if (left <= 0) return false;
@@ -212,6 +219,10 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_
         at = begin - place;
         w.enter(place);
         found = w.t1 > w.t0;
+        if (!found) {                // another team's, or nothing but the places before its tiles
+          at += w.places();
+          found = w.next(p, units);
+        }
       }
       before += __shfl_sync(0xffffffffu, incl, 31);
       if (last < (int64_t)before * units) return found;      // the same for all warps, which meet above
@@ -264,33 +275,39 @@ __device__ __forceinline__ void own_row(const DecodeParams& p, int b, int h, int
   }
 }
 
-// Copies a tile's rows one by one: the ones that a page's end divides, the last ones of a sequence, its own row and the depth rows.
-// Lane l finds the K row (l < 16) or the V row of key first + l % 16; page0 and page1: the pages of the tile's first and last key.
+// Copies a tile's rows one by one: where a page ends in it, where a page is missing, and where the token's own row is.  Lane l finds the K row
+// (l < 16) or the V row of key l % 16; page0 and page1: the pages of the tile's first and last row.
 template <typename T, int D>
-__device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w, int h, bool write, int first, int page0, int page1, uint32_t slot, uint32_t* mask) {
+__device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w, int tile, int h, bool write, int page0, int page1, uint32_t slot, uint32_t* mask) {
   constexpr int kChunks = D / 8, kRows = 32 / kChunks, kCopies = kTile / kRows;
   const Sequence& s = w.s;
   const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
-  const int key = first + (lane & 15);
-  const bool of_v = lane >= 16, own = key >= s.held && key < s.len;
-  bool valid = key < s.keys;
+  const bool of_v = lane >= 16;
   const unsigned char* row = static_cast<const unsigned char*>(p.pages.k.ptr);
   int page = -1, slot_of = 0;
-  if (key < s.len) {
-    const int which = (int)p.pages.by_page.div((uint32_t)key);
-    if (p.pages.page_size < kTile) page = __ldg(p.pages.table + w.b * p.pages.table_stride + which);      // a tile may lie in more than two
-    else page = which == (int)p.pages.by_page.div((uint32_t)first) ? page0 : page1;
-    slot_of = key - which * p.pages.page_size;
-    valid = page >= 0 && page < p.pages.num_pages;
-    if (!valid) wrong(kBadPage);
-    else if (own) row = static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h);
-    else row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
-  } else if (valid) {
-    const int d = key - s.len, pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
-    row = of_v ? static_cast<const unsigned char*>(p.vd.ptr) + 2 * (p.vd.off(w.b, layer, h) + pos * p.vd_sp)
-               : static_cast<const unsigned char*>(p.kd.ptr) + 2 * (p.kd.off(w.b, layer, h) + pos * p.kd_sp);
+  bool valid, own = false;
+  if (tile < s.cached_tiles) {
+    const int key = tile * kTile + (lane & 15);
+    valid = key < s.len;
+    own = valid && key >= s.held;
+    if (valid) {
+      const int which = (int)p.pages.by_page.div((uint32_t)key);
+      if (p.pages.page_size < kTile) page = __ldg(p.pages.table + w.b * p.pages.table_stride + which);      // a tile may lie in more than two
+      else page = which == (int)p.pages.by_page.div((uint32_t)(tile * kTile)) ? page0 : page1;
+      slot_of = key - which * p.pages.page_size;
+      valid = page >= 0 && page < p.pages.num_pages;
+      own = own && valid;
+      if (!valid) wrong(kBadPage);
+      else if (own) row = static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h);
+      else row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
+    }
+  } else {
+    const int d = (tile - s.cached_tiles) * kTile + (lane & 15), pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
+    valid = d < s.depth;
+    if (valid) row = of_v ? static_cast<const unsigned char*>(p.vd.ptr) + 2 * (p.vd.off(w.b, layer, h) + pos * p.vd_sp)
+                          : static_cast<const unsigned char*>(p.kd.ptr) + 2 * (p.kd.off(w.b, layer, h) + pos * p.kd_sp);
   }
-  const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own && valid) & 0xffffu;
+  const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own) & 0xffffu;
   if (lane == 0) *mask = there;
   const unsigned long long at = reinterpret_cast<unsigned long long>(row);
 #pragma unroll 2
@@ -307,14 +324,14 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
   }
 }
 
-// A tile's K (or V) rows, each `stride` elements behind the one before.  `from`: this lane's chunk of the first copy's row, which goes to
-// `to`.  The rows of copy i swizzle as those of the first do, but for bits that are known of i.
-template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to, const void* from, int64_t stride) {
+// A tile's K (or V) rows, each `stride` elements behind the one before; from row `count` on zeros.  `from`: this lane's chunk of row `row`, which
+// is the first copy's and goes to `to`.  The rows of copy i swizzle as those of the first do, but for bits that are known of i.
+template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to, const void* from, int64_t stride, int row, int count) {
   constexpr int kRows = 32 / (D / 8), kCopies = kTile / kRows;
   const unsigned char* at = static_cast<const unsigned char*>(from);
 #pragma unroll
   for (int i = 0; i < kCopies; ++i, at += kRows * 2 * stride)
-    copy16((to ^ ((kV ? i * kRows & 7 : k_swizzle(i * kRows & 7)) << 4)) + i * kRows * D * 2, at, true);
+    copy16((to ^ ((kV ? i * kRows & 7 : k_swizzle(i * kRows & 7)) << 4)) + i * kRows * D * 2, at, row + i * kRows < count);
 }
 
 // Copies the tiles of one warp, ahead of their use.
@@ -340,7 +357,7 @@ template <typename T, int D> struct Loader {
     base = tile;
     page0 = page1 = -1;
     const int mine = tile + team * (int)(threadIdx.x & 31);
-    if (!more || mine >= w.t1 || mine * kTile >= w.s.len) return;
+    if (!more || mine >= w.t1 || mine >= w.s.cached_tiles) return;
     const int first = mine * kTile;
     const int* row = p.pages.table + w.b * p.pages.table_stride;
     page0 = __ldg(row + p.pages.by_page.div((uint32_t)first));
@@ -357,17 +374,34 @@ template <typename T, int D> struct Loader {
   __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, uint32_t* masks) {
     if (more) {
       const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
-      const int first = tile * kTile, h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
+      const int h = query_blocks == 1 ? w.unit : w.unit / query_blocks, of = team == 1 ? tile - base : (tile - base) / kWarps;
       const uint32_t slot = ring + stage * stage_bytes<D>();
-      const int row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
-      const int page = __shfl_sync(0xffffffffu, page0, team == 1 ? tile - base : (tile - base) / kWarps);
-      if (first + kTile <= w.s.held && row0 + kTile <= p.pages.page_size && page >= 0 && page < p.pages.num_pages) {
-        // sixteen rows of one page
-        if (lane == 0) masks[stage] = 0xffffu;
-        copy_rows<D, false>(slot + to_k, rotary::chunk_at(p.pages.k, p.pages.k.off(page, row0 + r, h), c), p.pages.k.st);
-        copy_rows<D, true>(slot + to_v, rotary::chunk_at(p.pages.v, p.pages.v.off(page, row0 + r, h), c), p.pages.v.st);
+      const int page = __shfl_sync(0xffffffffu, page0, of);
+      // rows that follow one another in memory: of one page, or depth rows of one position
+      View k = p.pages.k, v = p.pages.v;
+      int64_t of_k, of_v;
+      int count;
+      bool run;
+      if (tile < w.s.cached_tiles) {
+        const int first = tile * kTile, row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
+        count = min(w.s.len - first, kTile);
+        run = first + count <= w.s.held && row0 + count <= p.pages.page_size && page >= 0 && page < p.pages.num_pages;
+        of_k = k.off(page, row0 + r, h);
+        of_v = v.off(page, row0 + r, h);
       } else {
-        mixed_tile<T, D>(p, w, h, w.unit == h * query_blocks, first, page, __shfl_sync(0xffffffffu, page1, team == 1 ? tile - base : (tile - base) / kWarps), slot, masks + stage);
+        const int first = (tile - w.s.cached_tiles) * kTile, pos = (int)p.by_L.div((uint32_t)first), layer = first - pos * p.L;
+        count = min(w.s.depth - first, kTile);
+        run = layer + count <= p.L;
+        k = p.kd; v = p.vd;
+        of_k = k.off(w.b, layer + r, h) + pos * p.kd_sp;
+        of_v = v.off(w.b, layer + r, h) + pos * p.vd_sp;
+      }
+      if (run) {
+        if (lane == 0) masks[stage] = (1u << count) - 1;
+        copy_rows<D, false>(slot + to_k, rotary::chunk_at(k, of_k, c), k.st, r, count);
+        copy_rows<D, true>(slot + to_v, rotary::chunk_at(v, of_v, c), v.st, r, count);
+      } else {
+        mixed_tile<T, D>(p, w, tile, h, w.unit == h * query_blocks, page, __shfl_sync(0xffffffffu, page1, of), slot, masks + stage);
       }
       tile += team;
       settle(p, units, false);

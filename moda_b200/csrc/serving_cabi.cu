@@ -289,7 +289,7 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   }
   // the kernels count keys, and the tiles of one head of all sequences, in 31 bits
   const int64_t most_keys = (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L;
-  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 1 + paged::unit_cost(paged::kWarps)) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
+  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 2 + paged::unit_cost(paged::kWarps)) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
   const int n_sm = sm_count(prob->device);
