@@ -64,11 +64,11 @@ struct DecodeParams {
 
 template <typename T> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
 template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Two values as 16 bits each, and what that leaves over.
@@ -96,6 +96,10 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
 // elements of column l / 4 in rows 2 (l % 4) and the next.
 __device__ __forceinline__ void load_transposed(uint32_t (&x)[4], uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+}
+
+__device__ __forceinline__ void sts128(uint32_t at, const uint4& x) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
 template <int D> __host__ __device__ constexpr int stage_bytes() { return kTile * D * 2 * 2; }
@@ -241,50 +245,50 @@ __device__ __forceinline__ void locate_cluster(const DecodeParams& p, int units,
   w.cost = 0;
 }
 
-// The new token's own row of head h: turned, written to its place in the cache (page, slot) and to the copies, and the key to its
-// place in the tile in shared memory (row n of the tile at `tile_k`; the value is copied there like any other).
+// The new token's own row, row n of a tile that has been copied as it was given: turned there, and written to its place in the cache (page, and slot
+// in it) and to the copies.  cs: cosines and sines of its position, which is the queries'.
 template <typename T, int D>
-__device__ __forceinline__ void own_row(const DecodeParams& p, int b, int h, int page, int slot, int position, bool write, uint32_t tile_k, int n) {
+__device__ __forceinline__ void own_row(const DecodeParams& p, const Walk& w, int h, int page, bool write, uint32_t tile, int n, const float2* cs) {
   constexpr int C = D / 16;
   const int lane = threadIdx.x & 31, c = lane % C;
-  float2 cs[8];
-  if (p.rot.inv_freq != nullptr) rotary::item_cos_sin<C>(p.rot, lane, position, cs);
-  if (lane >= 2 * C) return;
-  const bool of_v = lane >= C;
-  const View& in = of_v ? p.v : p.k;
-  int c0, c1;
-  const bool turns = rotary::item_chunks(p.rot, c, c0, c1) && p.rot.inv_freq != nullptr && !of_v;
-  uint4 x = *rotary::chunk_at(in, in.off(b, 0, h), c0), y = *rotary::chunk_at(in, in.off(b, 0, h), c1);
-  if (turns) rotary::turn<T>(x, y, cs, p.rot.interleaved != 0);
-  if (write) {
-    const View &to = of_v ? p.pages.v : p.pages.k, &copy = of_v ? p.v_copy : p.k_copy;
-    *rotary::chunk_at(to, to.off(page, slot, h), c0) = x;
-    *rotary::chunk_at(to, to.off(page, slot, h), c1) = y;
-    if (copy.ptr != nullptr) {
-      *rotary::chunk_at(copy, copy.off(b, 0, h), c0) = x;
-      *rotary::chunk_at(copy, copy.off(b, 0, h), c1) = y;
+  if (lane < 2 * C) {
+    const bool of_v = lane >= C;
+    int c0, c1;
+    const bool turns = rotary::item_chunks(p.rot, c, c0, c1) && p.rot.inv_freq != nullptr && !of_v;
+    const uint32_t row = tile + (of_v ? kTile + n : n) * D * 2, swizzle = of_v ? n & 7 : k_swizzle(n);
+    uint4 x = lds128(row + ((c0 ^ swizzle) << 4)), y = lds128(row + ((c1 ^ swizzle) << 4));
+    if (turns) {
+      float2 mine[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[i] = cs[8 * c + i];
+      rotary::turn<T>(x, y, mine, p.rot.interleaved != 0);
+      sts128(row + ((c0 ^ swizzle) << 4), x);
+      sts128(row + ((c1 ^ swizzle) << 4), y);
+    }
+    if (write) {
+      const int slot = w.s.held - (int)p.pages.by_page.div((uint32_t)w.s.held) * p.pages.page_size;
+      const View &to = of_v ? p.pages.v : p.pages.k, &copy = of_v ? p.v_copy : p.k_copy;
+      *rotary::chunk_at(to, to.off(page, slot, h), c0) = x;
+      *rotary::chunk_at(to, to.off(page, slot, h), c1) = y;
+      if (copy.ptr != nullptr) {
+        *rotary::chunk_at(copy, copy.off(w.b, 0, h), c0) = x;
+        *rotary::chunk_at(copy, copy.off(w.b, 0, h), c1) = y;
+      }
     }
   }
-  if (!of_v) {
-    const uint32_t row = tile_k + n * D * 2;
-    auto put = [&](int chunk, const uint4& z) {
-      asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(row + ((chunk ^ k_swizzle(n)) << 4)), "r"(z.x), "r"(z.y), "r"(z.z), "r"(z.w) : "memory");
-    };
-    put(c0, x);
-    put(c1, y);
-  }
+  __syncwarp();
 }
 
 // Copies a tile's rows one by one: where a page ends in it, where a page is missing, and where the token's own row is.  Lane l finds the K row
 // (l < 16) or the V row of key l % 16; page0 and page1: the pages of the tile's first and last row.
-template <typename T, int D>
-__device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w, int tile, int h, bool write, int page0, int page1, uint32_t slot, uint32_t* mask) {
+template <int D>
+__device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w, int tile, int h, int page0, int page1, uint32_t slot, uint2* mask) {
   constexpr int kChunks = D / 8, kRows = 32 / kChunks, kCopies = kTile / kRows;
   const Sequence& s = w.s;
   const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
   const bool of_v = lane >= 16;
   const unsigned char* row = static_cast<const unsigned char*>(p.pages.k.ptr);
-  int page = -1, slot_of = 0;
+  int page = -1;
   bool valid, own = false;
   if (tile < s.cached_tiles) {
     const int key = tile * kTile + (lane & 15);
@@ -294,11 +298,11 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
       const int which = (int)p.pages.by_page.div((uint32_t)key);
       if (p.pages.page_size < kTile) page = __ldg(p.pages.table + w.b * p.pages.table_stride + which);      // a tile may lie in more than two
       else page = which == (int)p.pages.by_page.div((uint32_t)(tile * kTile)) ? page0 : page1;
-      slot_of = key - which * p.pages.page_size;
+      const int slot_of = key - which * p.pages.page_size;
       valid = page >= 0 && page < p.pages.num_pages;
       own = own && valid;
       if (!valid) wrong(kBadPage);
-      else if (own) row = static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h);
+      else if (own) row = of_v ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h) : static_cast<const unsigned char*>(p.k.ptr) + 2 * p.k.off(w.b, 0, h);
       else row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
     }
   } else {
@@ -308,19 +312,15 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
                           : static_cast<const unsigned char*>(p.kd.ptr) + 2 * (p.kd.off(w.b, layer, h) + pos * p.kd_sp);
   }
   const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own) & 0xffffu;
-  if (lane == 0) *mask = there;
+  if (its_own == 0 ? lane == 0 : lane == __ffs(its_own) - 1) *mask = make_uint2(there | (uint32_t)__ffs(its_own) << 16, page);
   const unsigned long long at = reinterpret_cast<unsigned long long>(row);
 #pragma unroll 2
   for (int i = 0; i < kCopies; ++i) {
     const int n = i * kRows + r;
     const bool ok = (there >> n) & 1u;
     const unsigned long long k = __shfl_sync(0xffffffffu, at, n) + c * 16, v = __shfl_sync(0xffffffffu, at, 16 + n) + c * 16;
-    if (!((its_own >> n) & 1u)) copy16(slot + n * D * 2 + ((c ^ k_swizzle(n)) << 4), reinterpret_cast<const void*>(k), ok);
+    copy16(slot + n * D * 2 + ((c ^ k_swizzle(n)) << 4), reinterpret_cast<const void*>(k), ok);
     copy16(slot + (kTile + n) * D * 2 + ((c ^ (n & 7)) << 4), reinterpret_cast<const void*>(v), ok);
-  }
-  if (its_own != 0) {
-    const int n = __ffs(its_own) - 1;
-    own_row<T, D>(p, w.b, h, __shfl_sync(0xffffffffu, page, n), __shfl_sync(0xffffffffu, slot_of, n), s.held, write, slot, n);
   }
 }
 
@@ -335,7 +335,7 @@ template <int D, bool kV> __device__ __forceinline__ void copy_rows(uint32_t to,
 }
 
 // Copies the tiles of one warp, ahead of their use.
-template <typename T, int D> struct Loader {
+template <int D> struct Loader {
   Walk w;
   int tile;                          // this warp's next one, of w
   int team, rank;                    // the team's size, this warp's place in it
@@ -347,6 +347,8 @@ template <typename T, int D> struct Loader {
 
   static constexpr int kChunks = D / 8;
 
+  // A unit's part is walked from its end: the token's own row comes first, and what is written for it is on its way before the rest.
+  __device__ __forceinline__ int from_end(int n) const { return w.t0 + w.t1 - 1 - n; }
   __device__ __forceinline__ void settle(const DecodeParams& p, int units, bool fetch) {      // at a tile of this warp, or at the end
     while (more && tile >= w.t1) {
       more = w.next(p, units);
@@ -357,8 +359,8 @@ template <typename T, int D> struct Loader {
     base = tile;
     page0 = page1 = -1;
     const int mine = tile + team * (int)(threadIdx.x & 31);
-    if (!more || mine >= w.t1 || mine >= w.s.cached_tiles) return;
-    const int first = mine * kTile;
+    if (!more || mine >= w.t1 || from_end(mine) >= w.s.cached_tiles) return;
+    const int first = from_end(mine) * kTile;
     const int* row = p.pages.table + w.b * p.pages.table_stride;
     page0 = __ldg(row + p.pages.by_page.div((uint32_t)first));
     page1 = __ldg(row + p.pages.by_page.div((uint32_t)min(first + kTile, w.s.len) - 1u));
@@ -370,26 +372,27 @@ template <typename T, int D> struct Loader {
     to_v = kTile * D * 2 + r * D * 2 + (c ^ r) * 16;
     settle(p, units, true);
   }
-  // Issues the copies of one tile (none at the end); `masks` in shared memory get a bit for each key that is there.
-  __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, uint32_t* masks) {
+  // Issues the copies of one tile (none at the end); `masks` in shared memory get a bit for each key that is there, and from bit 16 on
+  // the number, from 1, of the token's own, with its page.
+  __device__ __forceinline__ void issue(const DecodeParams& p, int units, int query_blocks, uint2* masks) {
     if (more) {
       const int lane = threadIdx.x & 31, r = lane / kChunks, c = lane % kChunks;
       const int h = query_blocks == 1 ? w.unit : w.unit / query_blocks, of = team == 1 ? tile - base : (tile - base) / kWarps;
       const uint32_t slot = ring + stage * stage_bytes<D>();
-      const int page = __shfl_sync(0xffffffffu, page0, of);
+      const int page = __shfl_sync(0xffffffffu, page0, of), at = from_end(tile);
       // rows that follow one another in memory: of one page, or depth rows of one position
       View k = p.pages.k, v = p.pages.v;
       int64_t of_k, of_v;
       int count;
       bool run;
-      if (tile < w.s.cached_tiles) {
-        const int first = tile * kTile, row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
+      if (at < w.s.cached_tiles) {
+        const int first = at * kTile, row0 = first - (int)p.pages.by_page.div((uint32_t)first) * p.pages.page_size;
         count = min(w.s.len - first, kTile);
         run = first + count <= w.s.held && row0 + count <= p.pages.page_size && page >= 0 && page < p.pages.num_pages;
         of_k = k.off(page, row0 + r, h);
         of_v = v.off(page, row0 + r, h);
       } else {
-        const int first = (tile - w.s.cached_tiles) * kTile, pos = (int)p.by_L.div((uint32_t)first), layer = first - pos * p.L;
+        const int first = (at - w.s.cached_tiles) * kTile, pos = (int)p.by_L.div((uint32_t)first), layer = first - pos * p.L;
         count = min(w.s.depth - first, kTile);
         run = layer + count <= p.L;
         k = p.kd; v = p.vd;
@@ -397,11 +400,11 @@ template <typename T, int D> struct Loader {
         of_v = v.off(w.b, layer + r, h) + pos * p.vd_sp;
       }
       if (run) {
-        if (lane == 0) masks[stage] = (1u << count) - 1;
+        if (lane == 0) masks[stage].x = (1u << count) - 1;
         copy_rows<D, false>(slot + to_k, rotary::chunk_at(k, of_k, c), k.st, r, count);
         copy_rows<D, true>(slot + to_v, rotary::chunk_at(v, of_v, c), v.st, r, count);
       } else {
-        mixed_tile<T, D>(p, w, tile, h, w.unit == h * query_blocks, page, __shfl_sync(0xffffffffu, page1, of), slot, masks + stage);
+        mixed_tile<D>(p, w, at, h, page, __shfl_sync(0xffffffffu, page1, of), slot, masks + stage);
       }
       tile += team;
       settle(p, units, false);
@@ -448,10 +451,11 @@ __device__ __forceinline__ void join_cluster(const DecodeParams& p, const Walk& 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(const __grid_constant__ DecodeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ uint32_t s_masks[kWarps][kStages];
+  __shared__ uint2 s_masks[kWarps][kStages];
   __shared__ float2 s_ml[kWarps][kQ];
   __shared__ float2 s_cs[D / 2];
   __shared__ float2 s_part_ml[kQ];
+  __shared__ Range s_range;                  // read at units' ends alone: not worth registers
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, g = lane >> 2, t = lane & 3;
   const int query_blocks = (p.G + kQ - 1) / kQ, units = p.H * query_blocks;
   const uint32_t ring = smem_u32(smem) + warp * kStages * stage_bytes<D>();
@@ -459,14 +463,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 
   grid_before();
   grid_started();
-  Range range{};
   Walk w;
   int64_t at = 0;                            // the place of the walk's unit in the row of all units
   int team = kWarps;
   if (p.cluster != 0) {
     locate_cluster(p, units, w);
   } else {
+    Range range;
     const bool work = locate(p, units, reinterpret_cast<int*>(s_acc), team, range, w, at);
+    if (lane == 0) s_range = range;          // the same from all warps, and read by the one that has written it
+    __syncwarp();
     if (!work) {
       if (lane == 0 && (team == 1 || warp == 0)) p.parts[warp * gridDim.x + blockIdx.x] = make_int2(0, team == 1 ? -1 : 0);
       return;
@@ -474,21 +480,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
   }
   const int rank = team == 1 ? 0 : warp;
   const uint32_t worker = team == 1 ? blockIdx.x * kWarps + warp : blockIdx.x;
-  Loader<T, D> loader;
+  Loader<D> loader;
   loader.start(p, units, team, rank, w, ring);
 
   // places of this lane's chunks in a stage: K of row g (even and odd j), V of row lane % 16, chunk lane / 16
   const uint32_t k_even = g * D * 2 + (t ^ k_swizzle(g)) * 16, k_odd = g * D * 2 + ((4 + t) ^ k_swizzle(g)) * 16;
   const uint32_t v_place = (kTile + lane % 16) * D * 2 + ((lane >> 4) ^ (lane & 7)) * 16;
   int stage = 0, turned_b = -1, tile = 0, h = 0, q0 = 0;
-  int2 part = make_int2(0, team == 1 ? -1 : 0);
   uint32_t qh[D / 32][4], ql[D / 32][4];     // this lane's part of the queries, in two 16-bit halves
   float m = 0.f, l = 0.f, acc[D / 8][4];
   float2* cs = team == 1 ? reinterpret_cast<float2*>(s_acc) + (1 + warp) * 64 : s_cs;      // behind what locate() may still be reading
   const int cs_first = team == 1 ? lane : tid;
   const double inv_freq = p.rot.inv_freq != nullptr && cs_first < p.rot.rot / 2 ? p.rot.inv_freq[cs_first] : 0.;
-  // What a unit begins with: its queries' rows, and cosines and sines of their position, one a thread (those of the unit before have been
-  // read: its parts have been joined).
+  // What a unit begins with: its queries' rows.
   auto fetch = [&]() {
     h = query_blocks == 1 ? w.unit : w.unit / query_blocks;
     q0 = (w.unit - h * query_blocks) * kQ;
@@ -499,10 +503,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) qh[j][e] = (&x.x)[e];
     }
-    if (turned_b != w.b)
-      for (int i = cs_first; i < p.rot.rot / 2; i += 32 * team)
-        cs[i] = rotary::cos_sin(p.rot, i == cs_first ? inv_freq : p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
-    turned_b = w.b;
   };
   // Steps 1 - kStages to -1 only copy.  A step's copies are issued between the scores' products and what waits for them, and at
   // one place, for the sake of the code's size: warps are few, and wait for instructions where a step has more of them.
@@ -590,23 +590,38 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             if (!whole) join_cluster<T, D>(p, w, h, q0, smem_u32(smem), smem_u32(s_part_ml));
             return;
           }
-          if (from_start && !to_end) {             // begun here: how many CTAs hold a part of it
-            const int64_t last = at + w.places() - 1;
-            uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
-            while (range.begin(worker + n) > last) --n;
-            while (range.begin(worker + n + 1) <= last) ++n;
-            part = make_int2(w.b * units + w.unit, ((int)n + 1) * (team == 1 ? -1 : 1));
+          int2* const mine = p.parts + (team == 1 ? warp * gridDim.x : 0) + blockIdx.x;
+          if (!to_end) {                           // the last one of the range; begun here: how many teams hold a part of it
+            if (lane == 0 && rank == 0) {
+              int2 part = make_int2(0, team == 1 ? -1 : 0);
+              if (from_start) {
+                const Range range = s_range;
+                const int64_t last = at + w.places() - 1;
+                uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
+                while (range.begin(worker + n) > last) --n;
+                while (range.begin(worker + n + 1) <= last) ++n;
+                part = make_int2(w.b * units + w.unit, ((int)n + 1) * (team == 1 ? -1 : 1));
+              }
+              *mine = part;
+            }
+            return;
           }
           at += w.places();
           if (!w.next(p, units)) {
-            if (lane == 0 && rank == 0) p.parts[(team == 1 ? warp * gridDim.x : 0) + blockIdx.x] = part;
+            if (lane == 0 && rank == 0) *mine = make_int2(0, team == 1 ? -1 : 0);
             return;
           }
           fetch();
         }
         const bool row_there = q0 + g < p.G;
-        if (team == 1) __syncwarp();
-        else if (p.rot.inv_freq != nullptr) __syncthreads();
+        if (p.rot.inv_freq != nullptr) {     // one cosine and sine a thread, while the first copies are on the way
+          if (turned_b != w.b)               // those of the unit before have been read: its parts have been joined
+            for (int i = cs_first; i < p.rot.rot / 2; i += 32 * team)
+              cs[i] = rotary::cos_sin(p.rot, i == cs_first ? inv_freq : p.rot.inv_freq[i], p.k.ptr != nullptr ? w.s.held : w.s.held - 1);
+          turned_b = w.b;
+          if (team == 1) __syncwarp();
+          else __syncthreads();
+        }
 #pragma unroll
         for (int j = 0; j < D / 32; ++j) {
           const int chunk = 4 * j + t;
@@ -647,8 +662,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
       }
       copies_wait<kStages - 2>();
       __syncwarp();                          // the other lanes' copies, and the mask; and all lanes have read the tile before
-      mask = s_masks[warp][stage];
+      mask = s_masks[warp][stage].x;
       slot = ring + stage * stage_bytes<D>();
+      if (mask >> 16) {
+        own_row<T, D>(p, w, h, (int)s_masks[warp][stage].y, q0 == 0, slot, (int)(mask >> 16) - 1, cs);
+        mask &= 0xffffu;
+      }
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
