@@ -22,6 +22,7 @@
 //  - Eight query rows leave the lower half of the 16-row operand free.  It holds what rounding the upper half to 16
 //    bits has left over: the rotated query's remainder (the query is turned here, in 32 bits, without rounding), and that of
 //    the probabilities.  So neither is rounded to fewer than 16 significant bits, at no cost.
+//  - In fp16 probabilities are held times 2^15: 65536 keys of 2^-26 beside one of 1 are not to vanish below the type's range.
 #pragma once
 #include "rotary_kernels.cuh"
 
@@ -58,8 +59,9 @@ struct DecodeParams {
   // scratch where units are divided over all CTAs
   int2* parts;                     // [kWarps][CTA], of a CTA's one team or four: unit that it begins and others go on with, and how many hold a part
                                    // (none: 0; with four teams the numbers are negative, none: -1)
-  float2* ml;                      // [team][2][kQ]: maximum and sum; part 0 goes on from the team before, part 1 begins here
-  float* acc;                      // [team][2][kQ][D]
+  int rows;                        // min(G, kQ)
+  float2* ml;                      // [team][2][rows]: maximum and sum; part 0 goes on from the team before, part 1 begins here
+  float* acc;                      // [team][2][rows][D]
 };
 
 template <typename T> __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1);
@@ -71,9 +73,14 @@ template <> __device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Two values as 16 bits each, and what that leaves over.
+// What the exponents of probabilities are lifted by (the maximum m of a part is the true one less this).
+template <typename T> struct Lift { static constexpr float value = 0.f; };
+template <> struct Lift<__half> { static constexpr float value = 15.f; };
+// Two values as 16 bits each, and what that leaves over.  (A turned fp16 query may be larger than fp16: the upper half is its largest value then.)
+template <typename T> __device__ __forceinline__ float largest(float a) { return a; }
+template <> __device__ __forceinline__ float largest<__half>(float a) { return fminf(fmaxf(a, -65504.f), 65504.f); }
 template <typename T> __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = Pack<T>::pack(a, b);
+  hi = Pack<T>::pack(largest<T>(a), largest<T>(b));
   const float2 r = Pack<T>::unpack(hi);
   lo = Pack<T>::pack(a - r.x, b - r.y);
 }
@@ -426,19 +433,33 @@ __device__ __forceinline__ void join_cluster(const DecodeParams& p, const Walk& 
     if (q0 + r >= p.G) break;
     float top = -INFINITY, sum = 0.f;
     float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = 0; c < p.cluster; ++c) {
-      uint32_t at;
-      float2 x;
-      float4 y;
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ml + r * 8), "r"(c));
-      asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
-      asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(acc + (r * D + d) * 4), "r"(c));
-      asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w) : "r"(at) : "memory");
-      const float now = fmaxf(top, x.x), base = now == -INFINITY ? 0.f : now, a = fast_exp2(top - base), b = fast_exp2(x.x - base);
-      sum = sum * a + x.y * b;
-      out = make_float4(out.x * a + y.x * b, out.y * a + y.y * b, out.z * a + y.z * b, out.w * a + y.w * b);
+    for (int c0 = 0; c0 < p.cluster; c0 += 8) {      // eight CTAs' parts on the way together
+      float2 x[8];
+      float4 y[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        x[c] = make_float2(-INFINITY, 0.f);
+        y[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c0 + c >= p.cluster) continue;
+        uint32_t at;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ml + r * 8), "r"(c0 + c));
+        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x[c].x), "=f"(x[c].y) : "r"(at) : "memory");
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(acc + (r * D + d) * 4), "r"(c0 + c));
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(y[c].x), "=f"(y[c].y), "=f"(y[c].z), "=f"(y[c].w) : "r"(at) : "memory");
+      }
+      float now = top;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) now = fmaxf(now, x[c].x);
+      const float base = now == -INFINITY ? 0.f : now, was = fast_exp2(top - base);
+      sum *= was;
+      out = make_float4(out.x * was, out.y * was, out.z * was, out.w * was);
       top = now;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float weight = fast_exp2(x[c].x - base);
+        sum = fmaf(x[c].y, weight, sum);
+        out = make_float4(fmaf(y[c].x, weight, out.x), fmaf(y[c].y, weight, out.y), fmaf(y[c].z, weight, out.z), fmaf(y[c].w, weight, out.w));
+      }
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     uint2* to = reinterpret_cast<uint2*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + r, h) + d));
@@ -523,7 +544,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
           if (team == 1) {
             if (row_there) {
               const float inv = l == 0.f ? 0.f : 1.f / l;
-              const int64_t at_row = ((int64_t)worker * 2 + (from_start ? 1 : 0)) * kQ + g;
+              const int64_t at_row = ((int64_t)worker * 2 + (from_start ? 1 : 0)) * p.rows + g;
               uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + g, h) + 2 * t));
 #pragma unroll
               for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
@@ -578,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
                 if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
               } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
-                const int64_t at_row = p.cluster != 0 ? r : ((int64_t)worker * 2 + (from_start ? 1 : 0)) * kQ + r;
+                const int64_t at_row = p.cluster != 0 ? r : ((int64_t)worker * 2 + (from_start ? 1 : 0)) * p.rows + r;
                 float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) to[e] = out[e];
@@ -695,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
     float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    top = fmaxf(top, m);
+    top = fmaxf(top - Lift<T>::value, m);
     const float base = top == -INFINITY ? 0.f : top;
     if (__any_sync(0xffffffffu, top > m)) {
       const float shrink = fast_exp2(m - base);
@@ -742,7 +763,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 5) join_kernel(const __grid_c
     const int b = id / units, u = id - b * units, h = u / query_blocks, row = (u - h * query_blocks) * kQ + r;
     if (row >= p.G) continue;
     const int64_t first = by_warps ? blockIdx.x * kWarps + k : blockIdx.x;      // the team
-    auto place = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * kQ + r; };
+    auto place = [&](int i) { return ((first + i) * 2 + (i == 0 ? 1 : 0)) * p.rows + r; };
     constexpr int kEach = D / 32;
     float top = -INFINITY, sum = 0.f, out[kEach] = {};
     for (int i0 = warp; i0 < n; i0 += kJoinAhead * kJoinWarps) {

@@ -120,11 +120,11 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
 }
 
 // How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
-// the width of its table.
+// the width of its table (and L depth rows).
 struct Division { int ctas, cluster; };
 Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
   const int64_t heads = (int64_t)pr->H * ((pr->G + paged::kQ - 1) / paged::kQ), units = pr->B * heads;
-  const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile), slots = (int64_t)n_sm * (pr->D == 128 ? paged::ctas_per_sm<128>() : paged::ctas_per_sm<64>());
+  const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile + (pr->L + paged::kTile - 1) / paged::kTile), slots = (int64_t)n_sm * (pr->D == 128 ? paged::ctas_per_sm<128>() : paged::ctas_per_sm<64>());
   int cluster = 1;
   while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
   if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
@@ -133,8 +133,9 @@ Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
 }
 // Scratch of an evenly divided call: which units are shared, their parts' maxima and sums, their parts.
 size_t parts_bytes(int n) { return ((size_t)n * paged::kWarps * sizeof(int2) + 255) & ~(size_t)255; }
-size_t ml_bytes(int n) { return (size_t)n * paged::kWarps * 2 * paged::kQ * sizeof(float2); }
-size_t decode_scratch(int n, int D) { return parts_bytes(n) + ml_bytes(n) + (size_t)n * paged::kWarps * 2 * paged::kQ * D * sizeof(float); }
+size_t rows_of_teams(int n, int G) { return (size_t)n * paged::kWarps * 2 * std::min(G, paged::kQ); }
+size_t ml_bytes(int n, int G) { return rows_of_teams(n, G) * sizeof(float2); }      // a multiple of 64, so that the parts are aligned
+size_t decode_scratch(int n, int G, int D) { return parts_bytes(n) + ml_bytes(n, G) + rows_of_teams(n, G) * D * sizeof(float); }
 
 template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, int device, cudaStream_t st) {
   auto kern = paged::decode_kernel<T, D>;
@@ -247,7 +248,7 @@ int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, const moda_
   const int n_sm = sm_count(prob->device);
   if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
   const Division div = divide(prob, (int64_t)cache->max_pages * cache->page_size, n_sm);
-  *bytes = div.cluster != 0 ? 0 : decode_scratch(div.ctas, prob->D);
+  *bytes = div.cluster != 0 ? 0 : decode_scratch(div.ctas, prob->G, prob->D);
   return MODA_OK;
 }
 
@@ -298,18 +299,18 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   const int n_cta = div.ctas;
   p.cluster = div.cluster;
   if (p.cluster == 0) {
-    if (workspace == nullptr || workspace_bytes < decode_scratch(n_cta, prob->D)) return MODA_ERR_WORKSPACE;
+    if (workspace == nullptr || workspace_bytes < decode_scratch(n_cta, prob->G, prob->D)) return MODA_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
   }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
   p.q = to_view(q); p.o = to_view(o); p.lse = lse;
-  p.B = prob->B; p.H = prob->H; p.G = prob->G;
+  p.B = prob->B; p.H = prob->H; p.G = prob->G; p.rows = std::min(prob->G, paged::kQ);
   p.k = to_view(own_key ? k : nullptr); p.v = to_view(own_key ? v : nullptr);
   p.k_copy = to_view(own_key ? k_copy : nullptr); p.v_copy = to_view(own_key ? v_copy : nullptr);
   p.scale_log2 = prob->scale * 1.4426950408889634f;
   p.parts = reinterpret_cast<int2*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + parts_bytes(n_cta));
-  p.acc = reinterpret_cast<float*>(ws + parts_bytes(n_cta) + ml_bytes(n_cta));
+  p.acc = reinterpret_cast<float*>(ws + parts_bytes(n_cta) + ml_bytes(n_cta, prob->G));
   g_last_launches = 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const bool bf = prob->dtype == MODA_BF16;

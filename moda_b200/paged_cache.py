@@ -53,8 +53,8 @@ def paged_moda_decode(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Ten
     also appended, as by ``paged_moda_append``; without them its row is the sequence's last), and the depth rows
     ``cached_k, cached_v``: ``[B, L, H, D]`` of its own position, or ``[B, P, L, H, D]`` of positions of its chunk, of which it sees the
     first ``depth_positions[b]`` (int32; chunk-visible).  With ``rotary`` ``q`` and ``k`` are turned at the token's position;
-    depth rows are used as they are.  ``record_k, record_v [B, 1, H, D]`` receive the token's row as written to the cache.  A
-    token that sees nothing gets ``o = 0``, ``lse = -inf``."""
+    depth rows are used as they are.  ``record_k, record_v [B, 1, H, D]`` (none of the rows that are read) receive the token's row as
+    written to the cache.  A token that sees nothing gets ``o = 0``, ``lse = -inf``."""
     r = _cabi.native().paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale,
                                     moda_group_num, rotary, record_k, record_v)
     return r if need_lse else r[0]

@@ -198,6 +198,35 @@ def test_large_scores(built_library):
         _check_decode(o, lse, q, caches, table, [n], D ** -0.5)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_many_small_probabilities_beside_a_large_one(built_library, dtype):
+    """60000 keys of e^-18 each: 9e-4 together, and each below 2^-25, fp16's smallest step.  Their values are all there is to the result."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(18)
+    n, H, G, D, page = 60000, 1, 2, 64, 64
+    caches, table, lens = _pool(gen, dtype, [n], 0, page, H, D)
+    j = torch.arange(n, device=DEV)
+    caches[0][table[0, j // page].long(), j % page] = torch.where(j == 31234, 0.0, -2.25)[:, None, None].expand(n, H, D).to(dtype)
+    caches[1][table[0, j // page].long(), j % page] = torch.where(j == 31234, 0.0, 1.0)[:, None, None].expand(n, H, D).to(dtype)
+    q = torch.ones(1, G, H, D, device=DEV, dtype=dtype)
+    o, lse = M.paged_moda_decode(q, *caches, table, lens, moda_group_num=G, need_lse=True)
+    assert abs(o[0, 0, 0, 0].item() - 9.1e-4) < 1e-5
+    _check_decode(o, lse, q, caches, table, [n], D ** -0.5)
+
+
+def test_turned_queries_beyond_fp16(built_library):
+    """Pairs of 60000 turn to up to 84853, which fp16 does not hold; the score of small keys is an ordinary number."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(19)
+    lens, H, G, D, page = [50, 7, 300], 2, 2, 64, 16
+    caches, table, n = _pool(gen, HF, lens, 1, page, H, D)
+    caches[0].mul_(1e-5)
+    rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0])
+    q = torch.where(torch.rand(3, G, H, D, generator=gen, device=DEV) < 0.5, -60000.0, 60000.0).half()
+    o, lse = M.paged_moda_decode(q, *caches, table, n, rotary=rotary, moda_group_num=G, need_lse=True)
+    _check_decode(o, lse, q, caches, table, lens, D ** -0.5, None, (rotary, n.long() - 1))
+
+
 def test_nan_stays_where_it_belongs(built_library):
     """A NaN key of one sequence's head spoils that head's result and no other."""
     import moda_b200 as M
