@@ -6,11 +6,12 @@
 // flops for 4 D bytes, so the call is bound by memory up to G = 64 or so, and what the kernel is built for is to
 // have bytes on the way at all times:
 //
-//  - The work, 16-key tiles of every (b, h) in one row, is divided evenly between the CTAs by the lengths on
+//  - The work, 16-key tiles of every (b, h) in one row, is divided evenly between the CTAs (or their warps) by the lengths on
 //    the device (nothing is known on the host, and a captured call must follow new lengths).  A CTA walks its
 //    range, which may end one unit, hold several and begin another.  A unit that lies in one CTA's range is
-//    written at once, the others' parts are joined by a second, dependent launch.
-//  - A warp takes every fourth tile of the CTA's range and copies it, asynchronously, into slots of shared memory of its
+//    written at once, the others' parts are joined by a second, dependent launch.  Where the width of the table says that no
+//    sequence is long and there are few of them, a unit goes to a cluster of CTAs instead, and all is done in one launch.
+//  - A warp takes every fourth tile of a unit's part and copies it, asynchronously, into slots of shared memory of its
 //    own, kStages - 1 tiles ahead and across the ends of units: warps do not wait for one another.  An instruction copies
 //    whole rows (512 bytes in one piece where a page holds its heads one after another).  Measured on 1 GB: 7.0 TB/s, against
 //    5.0 where a lane copies the chunks that it will multiply, eight rows and 64 bytes of each an instruction.
@@ -78,12 +79,14 @@ template <typename T> struct Lift { static constexpr float value = 0.f; };
 template <> struct Lift<__half> { static constexpr float value = 15.f; };
 // Two values as 16 bits each, and what that leaves over.  (A turned fp16 query may be larger than fp16: the upper half is its largest value then.)
 template <typename T> __device__ __forceinline__ float largest(float a) { return a; }
-template <> __device__ __forceinline__ float largest<__half>(float a) { return fminf(fmaxf(a, -65504.f), 65504.f); }
+template <> __device__ __forceinline__ float largest<__half>(float a) { return isinf(a) ? a : fminf(fmaxf(a, -65504.f), 65504.f); }
 template <typename T> __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = Pack<T>::pack(largest<T>(a), largest<T>(b));
   const float2 r = Pack<T>::unpack(hi);
   lo = Pack<T>::pack(a - r.x, b - r.y);
 }
+// A sum over the two halves.  What is left over is 0 or of either sign: against an infinite key or value it says nothing.
+__device__ __forceinline__ float both(float hi, float lo) { return fabsf(lo) < INFINITY ? hi + lo : hi; }
 // 16 bytes from global memory to shared memory; !valid: zeros, and nothing is read.
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool valid) {
   asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" :: "r"(to), "l"(from), "r"(valid ? 16 : 0) : "memory");
@@ -96,9 +99,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t at) {
   return x;
 }
 
-// A tile in shared memory: 16 rows of K, 16 of V.  Chunk c (16 bytes) of row r is at place c ^ k_swizzle(r) of its row, or c ^ (r & 7):
-// the eight lanes that an access takes together then meet all banks, for the copies (chunks of one row) as for the reads
-// (K: chunks 4 j + t of two neighbouring rows g; V: one chunk of eight rows).
 // Four 8 x 8 matrices of 16-bit values, transposed: lane l gives the address of row l % 8 of matrix l / 8, and gets of each matrix the
 // elements of column l / 4 in rows 2 (l % 4) and the next.
 __device__ __forceinline__ void load_transposed(uint32_t (&x)[4], uint32_t at) {
@@ -109,6 +109,9 @@ __device__ __forceinline__ void sts128(uint32_t at, const uint4& x) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
 }
 
+// A tile in shared memory: 16 rows of K, 16 of V.  Chunk c (16 bytes) of row r is at place c ^ k_swizzle(r) of its row, or c ^ (r & 7):
+// the eight lanes that an access takes together then meet all banks, for the copies (chunks of one row) as for the reads
+// (K: chunks 4 j + t of two neighbouring rows g; V: one chunk of eight rows).
 template <int D> __host__ __device__ constexpr int stage_bytes() { return kTile * D * 2 * 2; }
 __host__ __device__ constexpr int k_swizzle(int r) { return ((r & 1) << 2) | ((r >> 1) & 3); }
 constexpr int kStages = 3;
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
               uint32_t* to = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(p.o.ptr) + 2 * (p.o.off(w.b, q0 + g, h) + 2 * t));
 #pragma unroll
               for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
-                const float x = acc[n][0] + acc[n][2], y = acc[n][1] + acc[n][3];
+                const float x = both(acc[n][0], acc[n][2]), y = both(acc[n][1], acc[n][3]);
                 if (whole) to[4 * n] = Pack<T>::pack(x * inv, y * inv);
                 else *reinterpret_cast<float2*>(p.acc + at_row * D + 8 * n + 2 * t) = make_float2(x, y);
               }
@@ -564,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 #pragma unroll
               for (int n = 0; n < D / 8; ++n) {      // elements 8 n + 2 t and the next
                 float* to = reinterpret_cast<float*>(part_at<D>(s_acc, warp, g, 2 * n + (t >> 1))) + (t & 1) * 2;
-                *reinterpret_cast<float2*>(to) = make_float2(acc[n][0] + acc[n][2], acc[n][1] + acc[n][3]);
+                *reinterpret_cast<float2*>(to) = make_float2(both(acc[n][0], acc[n][2]), both(acc[n][1], acc[n][3]));
               }
             }
             __syncthreads();
@@ -706,7 +709,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int nt = i >> 1, e = i & 1;
-      x[i] = ((s[nt][e] + s[nt][2 + e]) + (s2[nt][e] + s2[nt][2 + e])) * p.scale_log2;
+      x[i] = both(s[nt][e] + s2[nt][e], s[nt][2 + e] + s2[nt][2 + e]) * p.scale_log2;
     }
     if (mask != 0xffffu) {
 #pragma unroll

@@ -287,6 +287,8 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
     p.by_L = rotary::FastDiv((uint32_t)prob->L);
   } else if (prob->L > 0) {
     return MODA_ERR_NULL;
+  } else {
+    p.kd = p.vd = View{p.pages.k.ptr, 0, 0, 0};      // no row of it is read
   }
   // the kernels count keys, and the tiles of one head of all sequences, in 31 bits
   const int64_t most_keys = (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L;

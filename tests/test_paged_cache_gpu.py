@@ -240,6 +240,34 @@ def test_nan_stays_where_it_belongs(built_library):
     assert not o[0, :, 0].isnan().any() and not o[1].isnan().any() and not lse[1].isnan().any()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("turned", [False, True])
+def test_infinite_keys_and_values(built_library, dtype, turned):
+    """An infinite element of a key makes its score infinite, of either sign: +inf gives NaN, as the quotient inf / inf does, -inf leaves the
+    key out.  An infinite value makes its element of the result infinite.  No other sequence, head or element notices."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(20)
+    lens, H, G, D, page = [40, 40, 40, 40], 2, 2, 64, 16
+    caches, table, n = _pool(gen, dtype, lens, 0, page, H, D)
+    q = _rand(gen, dtype, 4, G, H, D).abs() + 0.25
+    rotary = M.Rotary(M.rotary_frequencies(16, device=DEV)[0]) if turned else None      # the elements concerned do not turn
+    at = table[:, 1].long()
+    caches[0][at[0], 3, 1, 40] = float("inf")
+    caches[0][at[1], 3, 1, 40] = float("-inf")
+    caches[1][at[2], 3, 1, 40] = float("inf")
+    o, lse = M.paged_moda_decode(q, *caches, table, n, rotary=rotary, moda_group_num=G, need_lse=True)
+    assert o[0, :, 1].isnan().all()
+    assert (o[2, :, 1, 40] == float("inf")).all()
+    clean = [c.clone() for c in caches]
+    clean[0][at[0], 3, 1, 40] = clean[1][at[2], 3, 1, 40] = 0
+    clean[0][at[1], 3, 1, 40] = -60000.0                    # far enough below: its probability is 0 too
+    want, want_lse = M.paged_moda_decode(q, *clean, table, n, rotary=rotary, moda_group_num=G, need_lse=True)
+    same = torch.ones_like(o, dtype=torch.bool)
+    same[0, :, 1] = same[2, :, 1, 40] = False
+    assert torch.equal(o[same], want[same])
+    assert torch.equal(lse[1:], want_lse[1:]) and torch.equal(lse[0, :, 0], want_lse[0, :, 0])
+
+
 def test_bad_tables_and_lengths_are_left_out_and_recorded(built_library):
     """Page numbers outside the pool: the kernels look at each before they use it.  Lengths outside the table: bounded by it."""
     import moda_b200 as M
@@ -265,6 +293,12 @@ def test_bad_tables_and_lengths_are_left_out_and_recorded(built_library):
                             torch.tensor([4, 0], dtype=torch.int32, device=DEV))
         assert M.device_status() == (2 << 8 | 1)
         assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(caches, before))
+    depth = [_rand(gen, BF, 2, 3, 2, H, D) for _ in range(2)]
+    for bad, seen in ((4, 3), (-1, 0)):
+        positions = torch.tensor([bad, 2], dtype=torch.int32, device=DEV)
+        o, lse = M.paged_moda_decode(q, *caches, table, n, cached_k=depth[0], cached_v=depth[1], depth_positions=positions, moda_group_num=G, need_lse=True)
+        assert M.device_status() == (2 << 8 | 2)
+        _check_decode(o, lse, q, caches, table, lens, D ** -0.5, depth, seen=[seen, 2])
     room = table.shape[1] * page
     full, ftable, _ = _pool(gen, BF, [room, room], 0, page, H, D)
     for bad, seen in (([-5, room], [0, room]), ([room + 1, 3], [room, 3]), ([2 ** 31 - 1, -2 ** 31], [room, 0])):
@@ -319,17 +353,26 @@ def test_refusals_on_the_gpu(built_library):
     assert e.value.status == 2
 
 
-def test_captured_steps_follow_the_lengths(built_library):
-    """A decoding step is captured once and replayed while the sequences grow; two captured graphs and an eager call share nothing."""
+@pytest.mark.parametrize("lens", [[900, 0, 33], [9000, 5, 20]])       # short enough for clusters; divided evenly
+def test_captured_steps_follow_the_lengths(built_library, lens):
+    """A decoding step is captured once and replayed while the sequences grow, behind a copy and behind another stream's work; two
+    captured graphs and an eager call share nothing."""
     import moda_b200 as M
     gen = torch.Generator(device=DEV).manual_seed(15)
     H, G, D, page, B = 2, 4, 128, 16, 3
-    lens = [900, 0, 33]
     caches, table, n = _pool(gen, BF, lens, 12, page, H, D)
     rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0])
     q, k, v = _rand(gen, BF, B, G, H, D), _rand(gen, BF, B, 1, H, D), _rand(gen, BF, B, 1, H, D)
 
+    other, given, also = torch.cuda.Stream(), q.clone(), torch.zeros(1 << 16, device=DEV)
+
     def step():
+        here = torch.cuda.current_stream()
+        other.wait_stream(here)
+        with torch.cuda.stream(other):
+            also.add_(1)
+        q.copy_(given)                                                   # a copy, not a kernel, is what comes before
+        here.wait_stream(other)
         r = M.paged_moda_decode(q, *caches, table, n, k, v, rotary=rotary, moda_group_num=G, need_lse=True)
         n.add_(1)
         return r
@@ -347,7 +390,7 @@ def test_captured_steps_follow_the_lengths(built_library):
     torch.cuda.current_stream().wait_stream(side)
     assert n.tolist() == [x + 1 for x in lens]
     for i in range(5):
-        for x in (q, k, v):
+        for x in (given, k, v):
             x.copy_(_rand(gen, BF, *x.shape))
         graphs[i % 2].replay()
         torch.cuda.synchronize()
