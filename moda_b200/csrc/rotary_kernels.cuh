@@ -5,9 +5,9 @@
 // round, by -a.  Pairs are elements (i, i + rot / 2) ("half") or (2 i, 2 i + 1) ("interleaved") of the first
 // rot elements of a head; the others pass through.
 //
-// The angle is reduced in whole turns and in integers: f / 2 pi modulo 1 as a 64-bit fraction, times p with the
-// product's overflow dropped, is p f / 2 pi modulo 1, since what overflows are whole turns.  A position of
-// 2^31 leaves 2^-33 of a turn of error, where an angle in 32-bit floating point is off by whole radians.
+// The angle is reduced in whole turns and in integers: f / 2 pi modulo 1 as a 64-bit fraction (from a product in two
+// parts), times p with the product's overflow dropped, is p f / 2 pi modulo 1, since what overflows are whole turns.  A position of
+// 2^31 leaves 2^-32 of a turn of error, where an angle in 32-bit floating point is off by whole radians.
 //
 // The operators move bytes: x is read and y written once.  A warp takes a token: every vector of
 // the token (G H query heads and H key heads) turns by the same angles, so a lane computes its share of the
@@ -46,9 +46,9 @@ struct Args {                // how vectors are turned
 // most an eighth of a turn (x = pi / 4), goes through the Taylor series in 64 bits (first terms left out: x^13 / 13! = 7e-12, x^12 / 12! =
 // 1.2e-10), so that the only error to speak of is the rounding to 32 bits at the end.  A lane does this once or twice a token.
 __device__ __forceinline__ float2 cos_sin(const Args& a, double f, long long pos) {
-  double turns = f * 0.15915494309189533577;               // 1 / 2 pi
-  turns -= floor(turns);
-  const unsigned long long step = (unsigned long long)(turns * 18446744073709551616.0);
+  constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;      // 1 / 2 pi
+  const double all = f * kHi, rest = fma(f, kLo, fma(f, kHi, -all));
+  const unsigned long long step = (unsigned long long)((all - floor(all)) * 18446744073709551616.0) + (unsigned long long)(long long)(rest * 18446744073709551616.0);
   const uint32_t turn = (uint32_t)((step * (unsigned long long)pos) >> 32);        // of a turn, times 2^32
   const uint32_t quarters = (turn + 0x20000000u) >> 30;
   const double x = (double)(int)(turn - (quarters << 30)) * 1.4629180792671596e-9, x2 = x * x;      // 2 pi / 2^32
