@@ -394,21 +394,23 @@ Pair rotary(const RotaryOp& op, const Tensor& q, const Tensor& k, const Tensor& 
 
 // The transposed map is the rotation by the negative angles, which is the same operator (and has a derivative of its own).
 struct MoDARotaryBackward : public Node {
-  RotaryOp op;
-  SavedVariable positions;
+  RotaryOp op;                         // without its frequencies, which are saved
+  SavedVariable positions, inv_freq;
   at::ScalarType dtype = at::kBFloat16;
   std::string name() const override { return "MoDARotaryBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
     positions.reset_data();
+    inv_freq.reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     variable_list out(next_edges().size());
     std::unique_lock<std::mutex> lock(mutex_);
     const Tensor at = positions.unpack();
+    RotaryOp back = op;
+    back.spec.inv_freq = inv_freq.unpack();
     lock.unlock();
     auto typed = [&](const Tensor& x) { return x.scalar_type() == dtype ? x : x.to(dtype); };
-    RotaryOp back = op;
     back.inverse = !op.inverse;
     const bool with_q = grads[0].defined() && task_should_compute_output(0);
     const bool with_k = grads.size() > 1 && grads[1].defined() && task_should_compute_output(1);
@@ -434,8 +436,10 @@ Pair rotary(const RotaryOp& op, const Tensor& q, const Tensor& k, const Tensor& 
   if (!grad) return r;
   std::shared_ptr<MoDARotaryBackward> node(new MoDARotaryBackward(), torch::autograd::deleteNode);
   node->op = op;
+  node->op.spec.inv_freq = Tensor();
   node->dtype = q.scalar_type();
   node->positions = SavedVariable(positions, false);
+  node->inv_freq = SavedVariable(op.spec.inv_freq, false);
   node->set_next_edges(torch::autograd::collect_next_edges(q, k));
   torch::autograd::set_history(r.q, node);
   if (k.defined()) torch::autograd::set_history(r.k, node);

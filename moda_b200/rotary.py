@@ -76,6 +76,7 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], rotary: Rotary,
     """Turns ``q [B, T*moda_group_num, H, D]`` and ``k [B, T, H, D]`` by their positions: ``(q, k)``, or ``q`` where ``k`` is None.
 
     ``positions``: None (token ``t`` stands at ``t``), the first token's position, or an int32 / int64 tensor ``[T]`` or
-    ``[B, T]``.  Differentiable in ``q`` and ``k``; the tensor of positions is used again in the backward and must not be changed before."""
+    ``[B, T]``.  Differentiable in ``q`` and ``k``; positions and frequencies are used again in the backward, which
+    notices if they have been changed in between."""
     q, k = _cabi.native().rotary(q, k, rotary, positions, moda_group_num)
     return q if k is None else (q, k)

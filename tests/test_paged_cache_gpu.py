@@ -312,6 +312,33 @@ def test_bad_tables_and_lengths_are_left_out_and_recorded(built_library):
         assert all(torch.equal(a.view(torch.int16), b.view(torch.int16)) for a, b in zip(full, before))
 
 
+@pytest.mark.parametrize("what", ["no room", "bad page", "negative length"])
+def test_a_row_without_a_place(built_library, what):
+    """The token's own row has nowhere to go: it is left out of the result too, nothing is written, and the other sequences go on."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    H, G, D, page = 2, 9, 64, 16
+    lens = [48, 33, 20]
+    caches, table, n = _pool(gen, BF, lens, 0, page, H, D)
+    table = table.clone()
+    if what == "bad page":
+        lens = [33, 33, 20]
+        table[0, 2] = -1
+    n = torch.tensor([-7 if what == "negative length" else lens[0], *lens[1:]], dtype=torch.int32, device=DEV)
+    held = {"no room": 48, "bad page": 32, "negative length": 0}[what]
+    before = [c.clone() for c in caches]
+    q, k, v = _rand(gen, BF, 3, G, H, D), _rand(gen, BF, 3, 1, H, D), _rand(gen, BF, 3, 1, H, D)
+    record = [torch.full((3, 1, H, D), 7.0, device=DEV, dtype=BF) for _ in range(2)]
+    o, lse = M.paged_moda_decode(q, *caches, table, n, k, v, moda_group_num=G, need_lse=True, record_k=record[0], record_v=record[1])
+    assert M.device_status() == (2 << 8 | (1 if what == "bad page" else 2))
+    _check_decode(o, lse, q, caches, table, [held, 34, 21], D ** -0.5)
+    assert (record[0][0] == 7).all() and (record[1][0] == 7).all() and torch.equal(record[0][1:], k[1:]) and torch.equal(record[1][1:], v[1:])
+    for c, old, new in zip(caches, before, (k, v)):
+        for b in (1, 2):
+            old[table[b, lens[b] // page].long(), lens[b] % page] = new[b, 0]
+        assert torch.equal(c.view(torch.int16), old.view(torch.int16))
+
+
 def test_offsets_past_32_bits(built_library):
     """A pool of more than 2^32 bytes: the sequences' pages are its first and its last ones."""
     import moda_b200 as M

@@ -170,13 +170,14 @@ def test_second_derivative_is_the_rotation_again(built_library):
     _check(dg, v, torch.arange(7, device=DEV)[None], rotary, "dg")
 
 
-def test_changed_positions_are_noticed(built_library):
+@pytest.mark.parametrize("which", ["positions", "inv_freq"])
+def test_changed_positions_or_frequencies_are_noticed(built_library, which):
     import moda_b200 as M
     q, k, rotary, _ = _case(M, 6, torch.bfloat16, 1, 7, 2, 1, 64, 64, False, 1.0)
     q.requires_grad_()
     at = torch.arange(7, device=DEV)
     y = M.rotary_embedding(q, None, rotary, positions=at)
-    at += 1
+    (at if which == "positions" else rotary.inv_freq).add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
 
