@@ -180,7 +180,7 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_
   const int tid = threadIdx.x, lane = tid & 31;
   int sum = 0, before = 0;           // tiles (places) of one unit of each sequence: below 2^31
   int64_t begin = 0, last = 0;       // of this team's range; of the CTA's last team's
-  bool found = false;
+  bool passed = false, found = false;      // the place has been; there is a unit for the team
   for (int pass = 0; pass < 2; ++pass)      // adds them up; finds the sequence that holds `begin`
     for (int base = 0; base < p.B; base += kThreads) {
       if (pass == 0 || p.B > kThreads) {
@@ -218,7 +218,8 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_
         if (lane >= o) incl += up;
       }
       const uint32_t here = __ballot_sync(0xffffffffu, begin < (int64_t)(before + incl) * units);
-      if (here != 0 && !found) {
+      if (here != 0 && !passed) {
+        passed = true;
         const int from = __ffs(here) - 1;
         int first = before + incl - mine, k = 0;      // of the lane's four sequences
         if (begin >= (int64_t)(first + x.x) * units) { first += x.x; k = 1;

@@ -67,6 +67,9 @@ DECODE = [  # dtype, lengths, H, G, D, L, page, heads
     (HF, [2500, 0, 3, 900], 5, 9, 128, 2, 32, True),           # few heads, too long for clusters
     (BF, [9000, 8999], 8, 8, 64, 11, 256, True),
     (BF, [1] * 1000, 3, 1, 64, 0, 8, True),
+    # more sequences than a CTA has threads, in units of single warps, of which many have none
+    (BF, [(61 * i) % 198 for i in range(299)], 2, 2, 128, 1, 16, True),
+    (HF, [(7 * i) % 90 for i in range(700)], 3, 1, 64, 3, 64, False),
 ]
 
 
