@@ -160,7 +160,11 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(const DecodeParams& p, int units) {
     if (left <= 0) return false;
-    if (++unit == units) { unit = 0; ++b; s = sequence(p, b); }
+    if (++unit == units) {
+      unit = 0;
+      if (++b >= p.B) return false;  // lengths that another stream changes meanwhile give no right result, but nothing is read outside
+      s = sequence(p, b);
+    }
     enter(0);
     return t1 > 0;                   // a range may end before the unit's first tile
   }
@@ -229,7 +233,7 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int units, int* s_
         w.b = __shfl_sync(0xffffffffu, base + lane * 4 + k, from);
         w.s = sequence(p, w.b);
         const int64_t off = begin - (int64_t)first * units;
-        w.unit = (int)quotient(off, (uint32_t)w.places());
+        w.unit = min((int)quotient(off, (uint32_t)w.places()), units - 1);
         const int place = (int)(off - (int64_t)w.unit * w.places());
         at = begin - place;
         w.enter(place);
@@ -623,8 +627,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 const Range range = s_range;
                 const int64_t last = at + w.places() - 1;
                 uint32_t n = (uint32_t)quotient(last - at, (uint32_t)min(range.each, (int64_t)0x7fffffff));      // the ranges are `each` long, or one more
-                while (range.begin(worker + n) > last) --n;
-                while (range.begin(worker + n + 1) <= last) ++n;
+                while (n > 0 && range.begin(worker + n) > last) --n;
+                while (worker + n + 1 < range.n && range.begin(worker + n + 1) <= last) ++n;
                 part = make_int2(w.b * units + w.unit, ((int)n + 1) * (team == 1 ? -1 : 1));
               }
               *mine = part;

@@ -162,6 +162,52 @@ def test_append(built_library, dtype, T, held, lengths, H, D, page, heads, rot, 
     assert M.device_status() == 0
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_drawn_calls(built_library, seed):
+    """Calls of all kinds: sizes, divisions of the work, page sizes, layouts, depth rows of one or several positions, own rows, rotations.  Two calls in
+    a row give the same bits (the second writes the same row again)."""
+    import random
+
+    import moda_b200 as M
+    rng = random.Random(seed)
+    for it in range(12):
+        dtype, D, H, G = rng.choice([BF, HF]), rng.choice([64, 128]), rng.choice([1, 2, 3, 5, 8, 13]), rng.choice([1, 2, 3, 4, 7, 8, 9, 16])
+        lens = rng.choice([
+            lambda: [int(2 ** rng.uniform(0, 15))],
+            lambda: [int(2 ** rng.uniform(0, 12)) - 1 for _ in range(rng.randint(2, 9))],
+            lambda: [rng.randint(0, rng.choice([1, 5, 40, 200])) for _ in range(rng.randint(50, 400))],
+            lambda: [int(2 ** rng.uniform(0, 11)) - 1 for _ in range(rng.randint(20, 60))],
+            lambda: [rng.randint(3000, 12000)] + [rng.choice([0, 1, 2]) for _ in range(rng.randint(0, 20))],
+        ])()
+        page, room, own = rng.choice([1, 3, 8, 16, 17, 24, 32, 64, 100, 256]), rng.choice([1, 1, 500, 3000]), rng.random() < 0.5
+        if len(lens) * (max(lens) + room) * H * D > 3e8:
+            room = 1
+            lens = lens[: max(1, int(3e8 / ((max(lens) + room) * H * D)))]
+        B = len(lens)
+        gen = torch.Generator(device=DEV).manual_seed(100 * seed + it)
+        caches, table, n = _pool(gen, dtype, lens, room, page, H, D, rng.random() < 0.6)
+        P, L, rot = rng.choice([0, 1, 1, 4]), rng.choice([1, 2, 7, 16, 33, 64]), rng.choice([0, 16, 64, D])
+        depth, seen, kw = None, None, {}
+        if P > 1:
+            depth, seen = tuple(_rand(gen, dtype, B, P, L + 2, H, D)[:, :, :L] for _ in range(2)), [rng.randint(0, P) for _ in range(B)]
+            kw["depth_positions"] = torch.tensor(seen, dtype=torch.int32, device=DEV)
+        elif P == 1:
+            depth = tuple(_rand(gen, dtype, B, L, H, D) for _ in range(2))
+        if depth is not None:
+            kw.update(cached_k=depth[0], cached_v=depth[1])
+        if rot:
+            kw["rotary"] = M.Rotary(M.rotary_frequencies(rot, device=DEV)[0], rng.random() < 0.5, rng.choice([1.0, 1.2]))
+        if own:
+            kw.update(k=_rand(gen, dtype, B, 1, H, D), v=_rand(gen, dtype, B, 1, H, D))
+        q, scale = _rand(gen, dtype, B, G, H, D), rng.choice([D ** -0.5, 0.3, -0.1])
+        o, lse = M.paged_moda_decode(q, *caches, table, n, **kw, scale=scale, moda_group_num=G, need_lse=True)
+        again = M.paged_moda_decode(q, *caches, table, n, **kw, scale=scale, moda_group_num=G, need_lse=True)
+        assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
+        turned = (kw["rotary"], n.long() - (0 if own else 1)) if rot else None
+        _check_decode(o, lse, q, caches, table, [x + own for x in lens], scale, depth, turned, seen)
+        assert M.device_status() == 0
+
+
 def test_strides_scale_and_views(built_library):
     """Caches that are slices of something larger, queries and rows that are views, shared pages, and scales of either sign."""
     import moda_b200 as M
