@@ -474,7 +474,8 @@ __device__ __forceinline__ void join_cluster(const DecodeParams& p, const Walk& 
     *to = make_uint2(Pack<T>::pack(out.x * inv, out.y * inv), Pack<T>::pack(out.z * inv, out.w * inv));
     if (d == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
   }
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");      // nobody leaves while it is read
+  // Nobody leaves while it is read.  What has been read has been used above; nothing else is waited for (a release would wait for o's stores).
+  asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory");
 }
 
 template <typename T, int D>

@@ -476,17 +476,18 @@ def test_captured_steps_follow_the_lengths(built_library, lens):
     assert M.device_status() == 0
 
 
-def test_calls_on_two_streams_at_once(built_library):
+def test_calls_on_several_streams_at_once(built_library):
     import moda_b200 as M
     gen = torch.Generator(device=DEV).manual_seed(16)
     H, G, D, page = 4, 4, 128, 64
     sets = []
-    for lens in ([6000, 10], [3000, 5000, 1]):
+    for lens in ([6000, 10], [3000, 5000, 1], [200, 90], [300]):         # divided evenly, and over clusters
         caches, table, n = _pool(gen, BF, lens, 0, page, H, D)
         sets.append((lens, caches, table, n, _rand(gen, BF, len(lens), G, H, D)))
     want = [M.paged_moda_decode(q, *caches, table, n, moda_group_num=G, need_lse=True) for _, caches, table, n, q in sets]
-    torch.cuda.synchronize()
-    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for (lens, caches, table, n, q), (o, lse) in zip(sets, want):
+        _check_decode(o, lse, q, caches, table, lens, D ** -0.5)
+    streams, got = [torch.cuda.Stream() for _ in sets], [[] for _ in sets]
     for _ in range(20):
         for i, (_, caches, table, n, q) in enumerate(sets):
             with torch.cuda.stream(streams[i]):
