@@ -282,7 +282,7 @@ int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, cons
  * more than the table covers.  Nothing that the call writes may be among the rows that it reads.
  * The results do not depend on scheduling.  workspace: caller-owned DEVICE scratch, 256-byte aligned,
  * contents undefined on entry and exit; calls that may overlap on the GPU need one each.  How many bytes (0: none, and
- * workspace may be NULL) depends on B, H, G, D, L and on how long the table lets a sequence be (max_pages, page_size).
+ * workspace may be NULL) depends on the device, on B, H, G, D, L and on how long the table lets a sequence be (max_pages, page_size).
  */
 int moda_b200_paged_decode_workspace_bytes(const moda_problem *prob, const moda_paged_cache *cache,
                                            size_t *bytes);

@@ -119,17 +119,66 @@ int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v,
   return MODA_OK;
 }
 
+// The decoding kernel, made ready once a device (the calls cost the host 0.4 us each).
+template <typename T, int D> int ready_decode(int device) {
+  static std::atomic<uint64_t> done{0};
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if ((done.load(std::memory_order_relaxed) & bit) != 0) return MODA_OK;
+  if (int rc = opt_in_smem(paged::decode_kernel<T, D>, paged::smem_bytes<D>())) return rc;
+  MODA_CUDA(cudaFuncSetAttribute(paged::decode_kernel<T, D>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return MODA_OK;
+}
+
+// How many clusters of 2^log_size CTAs the device, which is current, runs at once: fewer than its CTAs make, as a cluster lies in one
+// group of SMs and the groups differ in size (2 CTAs an SM: 14 clusters of 16, 33 of 8, 71 of 4).  Asked once a device.
+constexpr int kMostClusterLog = 4;
+template <int D> int clusters_at_once(int device, int log_size, int* out) {
+  static std::atomic<int> known[64][kMostClusterLog + 1];       // and one more; 0: not asked yet
+  if (device < 64) {
+    const int k = known[device][log_size].load(std::memory_order_relaxed);
+    if (k != 0) { *out = k - 1; return MODA_OK; }
+  }
+  if (int rc = ready_decode<__nv_bfloat16, D>(device)) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1u << log_size);
+  cfg.blockDim = dim3(paged::kThreads);
+  cfg.dynamicSmemBytes = paged::smem_bytes<D>();
+  cudaLaunchAttribute size{};
+  size.id = cudaLaunchAttributeClusterDimension;
+  size.val.clusterDim.x = 1u << log_size;
+  size.val.clusterDim.y = size.val.clusterDim.z = 1;
+  cfg.attrs = &size;
+  cfg.numAttrs = 1;
+  MODA_CUDA(cudaOccupancyMaxActiveClusters(out, paged::decode_kernel<__nv_bfloat16, D>, &cfg));
+  if (device < 64) known[device][log_size].store(*out + 1, std::memory_order_relaxed);
+  return MODA_OK;
+}
+
 // How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
 // the width of its table (and L depth rows).
 struct Division { int ctas, cluster; };
-Division divide(const moda_problem* pr, int64_t most_rows, int n_sm) {
+int divide(const moda_problem* pr, int64_t most_rows, Division* out) {
+  const int n_sm = sm_count(pr->device);
+  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
   const int64_t heads = (int64_t)pr->H * ((pr->G + paged::kQ - 1) / paged::kQ), units = pr->B * heads;
   const int64_t tiles = std::max<int64_t>(1, (most_rows + paged::kTile - 1) / paged::kTile + (pr->L + paged::kTile - 1) / paged::kTile), slots = (int64_t)n_sm * (pr->D == 128 ? paged::ctas_per_sm<128>() : paged::ctas_per_sm<64>());
-  int cluster = 1;
-  while (cluster < 16 && units * cluster * 2 <= slots && cluster * 2 * paged::kWarps <= tiles) cluster *= 2;
-  if (units <= slots && tiles <= 32 * cluster) return {(int)(units * cluster), cluster};
+  // clusters that have to wait for others cost a round: 16 sequences' heads of 2000 rows 14.4 us by 16, 9.5 by 8
+  int log_size = 0;
+  for (int next = 1; next <= kMostClusterLog && ((int64_t)paged::kWarps << next) <= tiles; ++next) {
+    int most = 0;
+    if (int rc = pr->D == 128 ? clusters_at_once<128>(pr->device, next, &most) : clusters_at_once<64>(pr->device, next, &most)) return rc;
+    if (units > most) break;
+    log_size = next;
+  }
+  const int cluster = 1 << log_size;
+  if (units <= slots && tiles <= 32 * cluster) {
+    *out = {(int)(units * cluster), cluster};
+    return MODA_OK;
+  }
   const int cost = paged::unit_cost(paged::kWarps), least = paged::least_places(paged::kWarps);
-  return {(int)std::min<int64_t>(slots, std::max<int64_t>(1, (units * (tiles + cost) + least - 1) / least)), 0};
+  *out = {(int)std::min<int64_t>(slots, std::max<int64_t>(1, (units * (tiles + cost) + least - 1) / least)), 0};
+  return MODA_OK;
 }
 // Scratch of an evenly divided call: which units are shared, their parts' maxima and sums, their parts.
 size_t parts_bytes(int n) { return ((size_t)n * paged::kWarps * sizeof(int2) + 255) & ~(size_t)255; }
@@ -140,14 +189,7 @@ size_t decode_scratch(int n, int G, int D) { return parts_bytes(n) + ml_bytes(n,
 template <typename T, int D> int decode(const paged::DecodeParams& p, int n_cta, int device, cudaStream_t st) {
   auto kern = paged::decode_kernel<T, D>;
   constexpr size_t smem = paged::smem_bytes<D>();
-  // once a device (the call costs the host 0.4 us)
-  static std::atomic<uint64_t> prepared{0};
-  const uint64_t bit = device < 64 ? 1ull << device : 0;
-  if ((prepared.load(std::memory_order_relaxed) & bit) == 0) {
-    if (int rc = opt_in_smem(kern, smem)) return rc;
-    MODA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    prepared.fetch_or(bit, std::memory_order_relaxed);
-  }
+  if (int rc = ready_decode<T, D>(device)) return rc;
   cudaError_t e;
   {
     prof::Scope ps(prof::kPagedDecode, st);
@@ -245,9 +287,10 @@ int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, const moda_
   if (bytes == nullptr || cache == nullptr) return MODA_ERR_NULL;
   if (int rc = check_sizes(prob)) return rc;
   if (cache->max_pages < 1 || cache->page_size < 1) return MODA_ERR_SHAPE;
-  const int n_sm = sm_count(prob->device);
-  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  const Division div = divide(prob, (int64_t)cache->max_pages * cache->page_size, n_sm);
+  DeviceGuard guard(prob->device);
+  if (!guard.ok) return cuda_fail(guard.err);
+  Division div;
+  if (int rc = divide(prob, (int64_t)cache->max_pages * cache->page_size, &div)) return rc;
   *bytes = div.cluster != 0 ? 0 : decode_scratch(div.ctas, prob->G, prob->D);
   return MODA_OK;
 }
@@ -295,9 +338,8 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 2 + paged::unit_cost(paged::kWarps)) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
-  const int n_sm = sm_count(prob->device);
-  if (n_sm <= 0) return cuda_fail(cudaErrorInvalidDevice);
-  const Division div = divide(prob, (int64_t)p.pages.max_pages * p.pages.page_size, n_sm);
+  Division div;
+  if (int rc = divide(prob, (int64_t)p.pages.max_pages * p.pages.page_size, &div)) return rc;
   const int n_cta = div.ctas;
   p.cluster = div.cluster;
   if (p.cluster == 0) {
