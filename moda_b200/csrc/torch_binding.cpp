@@ -450,6 +450,11 @@ struct PagedCache {                   // cache_k, cache_v, block_table, seq_lens
   Tensor k, v, table, lens;
   moda_paged_cache abi{};
 };
+// Autograd notices that what it has saved of these tensors is not what it was.
+void written(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* x : tensors)
+    if (x->defined() && !x->is_inference()) x->unsafeGetTensorImpl()->bump_version();
+}
 PagedCache as_paged(PyObject* const* a, int64_t B, int64_t H, int64_t D) {
   PagedCache c;
   for (int i = 0; i < 4; ++i) require_type(THPVariable_Check(a[i]), "moda_b200: the cache, its block table and seq_lens must be tensors");
@@ -759,6 +764,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     check_status(moda_b200_paged_append(&pr, T4(k).p(), T4(v).p(), &c.abi, lengths.defined() ? lengths.const_data_ptr<int32_t>() : nullptr,
                                         spec.inv_freq.defined() ? &rot : nullptr, c10::cuda::getCurrentCUDAStream().stream()),
                  "moda_b200_paged_append");
+    written({&c.k, &c.v});
   }
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
@@ -834,6 +840,7 @@ PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                         spec.inv_freq.defined() ? &rot : nullptr, T4(r.o).p(), r.lse.mutable_data_ptr<float>(),
                                         bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, c10::cuda::getCurrentCUDAStream().stream()),
                  "moda_b200_paged_decode");
+    if (k_.defined()) written({&c.k, &c.v, &rk, &rv});
   }
   return wrap(r);
   END_HANDLE_TH_ERRORS

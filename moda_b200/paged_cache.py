@@ -13,7 +13,7 @@ A pool of pages holds the rows of all sequences, ``[num_pages, page_size, H, D]`
         o = layer.cache.decode(q, block_table, seq_lens, k, v, depth=depth, record=True, moda_group_num=G, rotary=rotary)
     seq_lens += 1
 
-The functions do the same on tensors that the caller keeps.  Nothing here synchronises or reads lengths on the host, so
+The functions do the same on tensors that the caller keeps; what they write counts as modified in place.  Nothing here synchronises or reads lengths on the host, so
 that a step can be captured once and replayed while the sequences grow.  Rows that the tables or lengths
 put outside the pool are left out and recorded (``moda_b200.device_status()``).  There is no backward: inputs
 that require gradients are refused.

@@ -497,6 +497,40 @@ def test_calls_on_several_streams_at_once(built_library):
         assert all(torch.equal(w[0], g[0]) and torch.equal(w[1], g[1]) for g in gs)
 
 
+def test_writes_are_noticed_by_autograd(built_library):
+    import moda_b200 as M
+    H, G, D = 2, 2, 64
+    cache = M.PagedKVCache(4, 16, H, D, BF, "cuda")
+    cache.k.zero_()
+    cache.v.zero_()
+    table = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    n = torch.tensor([5], dtype=torch.int32, device="cuda")
+    q, k, record = (torch.randn(1, t, H, D, device="cuda").to(BF) for t in (G, 1, 1))
+    w = torch.ones(D, device="cuda", dtype=BF, requires_grad=True)
+
+    def saved(x):                            # the gradient of w reads x
+        return (x * w).sum()
+
+    y = [saved(x) for x in (cache.k, cache.v, record)]
+    cache.decode(q, table, n, moda_group_num=G)                           # reads only
+    for x in y:
+        x.backward(retain_graph=True)
+    for write in (lambda: cache.append(k, k, table, n), lambda: cache.decode(q, table, n, k, k, moda_group_num=G)):
+        y = [saved(x) for x in (cache.k, cache.v)]
+        write()
+        for x in y:
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                x.backward()
+    y = saved(record)
+    M.paged_moda_decode(q, cache.k, cache.v, table, n, k, k, moda_group_num=G, record_k=record, record_v=torch.empty_like(record))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():             # these tensors have no version
+        cache = M.PagedKVCache(4, 16, H, D, BF, "cuda")
+        cache.append(k, k, table, n)
+        cache.decode(q, table, n, k, k, moda_group_num=G)
+
+
 @pytest.mark.parametrize("chunk_visible,G", [(False, 2), (False, 1), (True, 4)])
 def test_generating_with_a_stack_of_layers(built_library, chunk_visible, G):
     """A prompt through the operators and its K/V into the caches, then tokens one by one: the attention of each layer at each new
