@@ -414,7 +414,7 @@ template <int D> struct Loader {
         of_k = k.off(w.b, layer + r, h) + pos * p.kd_sp;
         of_v = v.off(w.b, layer + r, h) + pos * p.vd_sp;
       }
-      if (run) {
+      if (__builtin_expect(run, 1)) {
         if (lane == 0) masks[stage].x = (1u << count) - 1;
         copy_rows<D, false>(slot + to_k, rotary::chunk_at(k, of_k, c), k.st, r, count);
         copy_rows<D, true>(slot + to_v, rotary::chunk_at(v, of_v, c), v.st, r, count);
@@ -535,14 +535,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
     }
   };
   // Steps 1 - kStages to -1 only copy.  A step's copies are issued between the scores' products and what waits for them, and at
-  // one place, for the sake of the code's size: warps are few, and wait for instructions where a step has more of them.
+  // one place, for the sake of the code's size: warps are few, and wait for instructions where a step has more of them.  For
+  // the same reason what is rare is marked so (64 sequences of up to 4096 rows: 63.5 us without, 62.2 with).
   fetch();
   for (int step = 1 - kStages;; ++step) {
     float s[2][4], s2[2][4];                 // two sums each: the products of one wait for one another
     uint32_t mask = 0, slot = 0;
     if (step >= 0) {
       bool begins = step == 0;
-      while (begins || tile >= w.t1) {
+      while (__builtin_expect(begins || tile >= w.t1, 0)) {
         if (!begins) {
           const bool row_there = q0 + g < p.G;
           // the warps' parts
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
       __syncwarp();                          // the other lanes' copies, and the mask; and all lanes have read the tile before
       mask = s_masks[warp][stage].x;
       slot = ring + stage * stage_bytes<D>();
-      if (mask >> 16) {
+      if (__builtin_expect(mask >> 16, 0)) {
         own_row<T, D>(p, w, h, (int)s_masks[warp][stage].y, q0 == 0, slot, (int)(mask >> 16) - 1, cs);
         mask &= 0xffffu;
       }
