@@ -10,7 +10,7 @@
 //    the device (nothing is known on the host, and a captured call must follow new lengths).  A CTA walks its
 //    range, which may end one unit, hold several and begin another.  A unit that lies in one CTA's range is
 //    written at once, the others' parts are joined by a second, dependent launch.  Where the width of the table says that no
-//    sequence is long and there are few of them, a unit goes to a cluster of CTAs instead, and all is done in one launch.
+//    sequence is long, all is done in one launch: few units go to a cluster of CTAs each, many short ones to single warps.
 //  - A warp takes every fourth tile of a unit's part and copies it, asynchronously, into slots of shared memory of its
 //    own, kStages - 1 tiles ahead and across the ends of units: warps do not wait for one another.  An instruction copies
 //    whole rows (512 bytes in one piece where a page holds its heads one after another).  Measured on 1 GB: 7.0 TB/s, against
@@ -36,6 +36,7 @@ constexpr int kQ = 8;              // query heads of a unit; more are further un
 // A team takes a unit: the four warps of a CTA, which divide its tiles; or, where there are many short units (kShort tiles on average),
 // each warp by itself, which has nothing to wait for.  1708 units of one tile, D = 128: 37 us by CTAs, 21 by warps.
 constexpr int kShort = 12, kWhole = 2 * kShort;
+constexpr int kByWarps = -1;
 // Tiles that a unit counts for beyond its own, where the work is divided: beginning and ending one takes a CTA about as long.  37
 // sequences of up to 1531 rows, 5 heads of 64 (units of 1 to 97 tiles): 23.2 us without, 18.0 with 4, 16.1 with 8, 16.8 with 16.
 __host__ __device__ constexpr int unit_cost(int team) { return team == 1 ? 2 : 8; }
@@ -56,7 +57,7 @@ struct DecodeParams {
   rotary::Args rot;                // of the queries and the own keys, at the last position of the sequence
   int B, H, G;
   float scale_log2;
-  int cluster;                     // 0: units are divided evenly over all CTAs; C: each unit over the C CTAs of a cluster
+  int cluster;                     // 0: units are divided evenly over all CTAs; C: each unit over the C CTAs of a cluster; kByWarps: whole units to warps
   // scratch where units are divided over all CTAs
   int2* parts;                     // [kWarps][CTA], of a CTA's one team or four: unit that it begins and others go on with, and how many hold a part
                                    // (none: 0; with four teams the numbers are negative, none: -1)
@@ -139,16 +140,23 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams& p, int b, bool 
   return s;
 }
 
-// A team's walk over its range: (sequence, unit of it, tiles [t0, t1) of the unit).  A unit takes `cost` places before its tiles.
+// A team's walk over its range: (sequence, unit of it, tiles [t0, t1) of the unit).  A unit takes `cost` places before its tiles.  No
+// cost: the range is one of whole units, which are counted (none where a cluster has its one unit).
 struct Walk {
   int cost;
   int b, unit;                       // unit: head * query blocks + query block
   Sequence s;
   int t0, t1;
-  int64_t left;                      // places of the range behind this unit
+  int64_t left;                      // places (units) of the range behind this unit
   __device__ __forceinline__ int places() const { return s.tiles + cost; }
   // The part of the unit from `place` on.  Short units of single warps stay whole, with the team that has their first place.
   __device__ __forceinline__ void enter(int place) {
+    if (cost == 0) {
+      --left;
+      t0 = 0;
+      t1 = s.tiles;
+      return;
+    }
     const int used = (int)min((int64_t)(places() - place), left);
     left -= used;
     t0 = max(place - cost, 0);
@@ -163,7 +171,7 @@ struct Walk {
     if (++unit == units) {
       unit = 0;
       if (++b >= p.B) return false;  // lengths that another stream changes meanwhile give no right result, but nothing is read outside
-      s = sequence(p, b);
+      s = sequence(p, b, cost == 0);
     }
     enter(0);
     return t1 > 0;                   // a range may end before the unit's first tile
@@ -258,6 +266,21 @@ __device__ __forceinline__ void locate_cluster(const DecodeParams& p, int units,
   w.t1 = (int)((uint32_t)w.s.tiles * (rank + 1) / p.cluster);
   w.left = 0;
   w.cost = 0;
+}
+
+// Whole units to warps: an even share of them, no unit being long.  False where there is none for this warp.
+__device__ __forceinline__ bool locate_units(const DecodeParams& p, int units, Walk& w) {
+  const uint32_t n = gridDim.x * kWarps, i = blockIdx.x * kWarps + threadIdx.x / 32;
+  const uint64_t all = (uint64_t)p.B * units;                     // below 2^31, n below 2^16
+  const uint32_t begin = (uint32_t)(all * i / n), end = (uint32_t)(all * (i + 1) / n);
+  if (begin == end) return false;
+  w.b = begin / units;
+  w.unit = begin - w.b * units;
+  w.s = sequence(p, w.b, w.unit == 0);
+  w.cost = 0;
+  w.left = end - begin;
+  w.enter(0);
+  return true;
 }
 
 // The new token's own row, row n of a tile that has been copied as it was given: turned there, and written to its place in the cache (page, and slot
@@ -496,8 +519,11 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
   Walk w;
   int64_t at = 0;                            // the place of the walk's unit in the row of all units
   int team = kWarps;
-  if (p.cluster != 0) {
+  if (p.cluster > 0) {
     locate_cluster(p, units, w);
+  } else if (p.cluster == kByWarps) {
+    team = 1;
+    if (!locate_units(p, units, w)) return;
   } else {
     Range range;
     const bool work = locate(p, units, reinterpret_cast<int*>(s_acc), team, range, w, at);
@@ -550,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
           l += __shfl_xor_sync(0xffffffffu, l, 1);
           l += __shfl_xor_sync(0xffffffffu, l, 2);
           const bool from_start = w.t0 == 0, to_end = w.t1 == w.s.tiles;
-          const bool whole = p.cluster != 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
+          const bool whole = p.cluster > 0 ? p.cluster == 1 : from_start && to_end;      // the same in all CTAs of a cluster, which meet below
           if (team == 1) {
             if (row_there) {
               const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -609,15 +635,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
                 for (int e = 0; e < kEach / 2; ++e) to[e] = packed[e];
                 if (d0 == 0) p.lse[((int64_t)w.b * p.G + q0 + r) * p.H + h] = top + log2f(sum);
               } else {                               // into scratch; a cluster's parts into each CTA's shared memory (its slots are free)
-                const int64_t at_row = p.cluster != 0 ? r : ((int64_t)worker * 2 + (from_start ? 1 : 0)) * p.rows + r;
-                float* to = (p.cluster != 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
+                const int64_t at_row = p.cluster > 0 ? r : ((int64_t)worker * 2 + (from_start ? 1 : 0)) * p.rows + r;
+                float* to = (p.cluster > 0 ? reinterpret_cast<float*>(smem) : p.acc) + at_row * D + d0;
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) to[e] = out[e];
-                if (d0 == 0) (p.cluster != 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
+                if (d0 == 0) (p.cluster > 0 ? s_part_ml : p.ml)[at_row] = make_float2(top, sum);
               }
             }
           }
-          if (p.cluster != 0) {
+          if (p.cluster > 0) {
             if (!whole) join_cluster<T, D>(p, w, h, q0, smem_u32(smem), smem_u32(s_part_ml));
             return;
           }
@@ -639,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
           }
           at += w.places();
           if (!w.next(p, units)) {
-            if (lane == 0 && rank == 0) *mine = make_int2(0, team == 1 ? -1 : 0);
+            if (p.cluster == 0 && lane == 0 && rank == 0) *mine = make_int2(0, team == 1 ? -1 : 0);
             return;
           }
           fetch();

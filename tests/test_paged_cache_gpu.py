@@ -476,6 +476,60 @@ def test_captured_steps_follow_the_lengths(built_library, lens):
     assert M.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype,lens,H,G,D,P,L,page", [
+    (BF, [(7 * i) % 100 for i in range(101)], 3, 4, 128, 1, 8, 16),
+    (HF, [i % 3 for i in range(230)], 2, 9, 64, 1, 3, 8),
+    (HF, [(11 * i) % 64 for i in range(1500)], 1, 2, 64, 0, 0, 64),
+    (BF, [i % 50 for i in range(150)], 4, 2, 128, 2, 5, 32),
+    (BF, [(5 * i) % 90 for i in range(120)], 4, 3, 64, 4, 64, 64),        # short but for its depth rows
+])
+def test_more_short_units_than_ctas(built_library, dtype, lens, H, G, D, P, L, page):
+    """Where the table lets no sequence be long and there are more units than CTAs, warps take whole units: nothing is joined."""
+    import moda_b200 as M
+    from moda_b200 import _cabi
+    gen = torch.Generator(device=DEV).manual_seed(18)
+    B = len(lens)
+    caches, table, n = _pool(gen, dtype, lens, 3, page, H, D)
+    rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0])
+    q, k, v = _rand(gen, dtype, B, G, H, D), _rand(gen, dtype, B, 1, H, D), _rand(gen, dtype, B, 1, H, D)
+    depth, seen, kw = None, None, {}
+    if P > 1:
+        depth, seen = [_rand(gen, dtype, B, P, L, H, D) for _ in range(2)], [i % (P + 1) for i in range(B)]
+        kw = dict(cached_k=depth[0], cached_v=depth[1], depth_positions=torch.tensor(seen, dtype=torch.int32, device=DEV))
+    elif P == 1:
+        depth = [_rand(gen, dtype, B, L, H, D) for _ in range(2)]
+        kw = dict(cached_k=depth[0], cached_v=depth[1])
+    _cabi.profile_begin()
+    o, lse = M.paged_moda_decode(q, *caches, table, n, moda_group_num=G, need_lse=True, **kw)
+    assert "paged_decode" in (ran := _cabi.profile_end()) and "paged_join" not in ran
+    _check_decode(o, lse, q, caches, table, lens, D ** -0.5, depth, seen=seen)
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = M.paged_moda_decode(q, *caches, table, n, k, v, rotary=rotary, moda_group_num=G, need_lse=True, **kw)
+        n.add_(1)
+    for i in range(2):
+        graph.replay()
+        now = [x + 1 + i for x in lens]
+        _check_decode(o, lse, q, caches, table, now, D ** -0.5, depth, (rotary, n.long() - 1), seen)
+    assert M.device_status() == 0
+
+    # a page of one sequence outside the pool, lengths of two outside the table
+    at = [i for i in range(B) if now[i] > 0]
+    broken, bad = table.clone(), n.clone()
+    broken[at[1], 0] = -1
+    o, lse = M.paged_moda_decode(q, *caches, broken, n, moda_group_num=G, need_lse=True, **kw)
+    assert M.device_status() == (2 << 8 | 1)
+    room = table.shape[1] * page
+    bad[at[0]], bad[at[-1]] = -3, room + 1
+    o2, lse2 = M.paged_moda_decode(q, *caches, table, bad, moda_group_num=G, need_lse=True, **kw)
+    assert M.device_status() == (2 << 8 | 2)
+    want, want_lse = M.paged_moda_decode(q, *caches, table, n, moda_group_num=G, need_lse=True, **kw)
+    for x, y, but in ((o, want, [at[1]]), (lse, want_lse, [at[1]]), (o2, want, [at[0], at[-1]]), (lse2, want_lse, [at[0], at[-1]])):
+        others = [i for i in range(B) if i not in but]
+        assert torch.equal(x[others], y[others])
+
+
 def test_calls_on_several_streams_at_once(built_library):
     import moda_b200 as M
     gen = torch.Generator(device=DEV).manual_seed(16)
