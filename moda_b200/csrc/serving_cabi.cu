@@ -52,14 +52,19 @@ int check_pages(const moda_problem* pr, const moda_paged_cache* c, paged::Pages*
 }
 
 // How the kernels that turn a token's vectors are divided: tokens a warp, vectors of a token that a warp takes, grid (tokens, shares of a
-// token's vectors).  A warp has 32 / (D / 16) vectors of a token side by side, or where there are so few of them as many tokens.
+// token's vectors).  A warp has 32 / (D / 16) vectors of a token side by side, or where there are so few of them as many tokens; more than
+// fill it at once where there would be more warps than run at once, since a warp that ends early costs more than one that takes
+// steps.  65536 tokens of 5 vectors of 64: 19.9 us, 28.9 without; of 9 of 128 53.4 and 57.9; 4096 of 4 of 128 would be 3.5 for 3.3.
 // A token that one warp can walk in a few steps stays whole (the sines are computed once); few tokens are shared by more warps, down to
 // one step of kBatch vectors a lane, until there are some 16 warps for each SM.
 struct TokenGrid { int tokens_a_warp, per_warp; dim3 grid; };
 TokenGrid token_grid(int64_t tokens, int vectors, int D, int n_sm) {
   TokenGrid r{1, 0, dim3()};
   int lanes = 32 / (D / 16);
-  while (r.tokens_a_warp < (D == 128 ? 2 : 4) && vectors * 2 <= lanes) { r.tokens_a_warp *= 2; lanes /= 2; }
+  while (r.tokens_a_warp < (D == 128 ? 2 : 4) && (vectors * 2 <= lanes || (vectors <= lanes * 3 && tokens > (int64_t)n_sm * 32 * r.tokens_a_warp))) {
+    r.tokens_a_warp *= 2;
+    lanes /= 2;
+  }
   const int step = lanes * rotary::kBatch, most = (vectors + step - 1) / step;
   const int64_t a_block = (int64_t)(rotary::kThreads / 32) * r.tokens_a_warp;
   const int64_t shares = std::min<int64_t>(most, std::max<int64_t>(1, (int64_t)n_sm * 16 / std::max<int64_t>(tokens, 1)));

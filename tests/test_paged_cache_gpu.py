@@ -162,6 +162,15 @@ def test_append(built_library, dtype, T, held, lengths, H, D, page, heads, rot, 
     assert M.device_status() == 0
 
 
+# more tokens than warps run at once: two or four a warp, in steps
+@pytest.mark.parametrize("dtype,T,held,lengths,H,D,page,heads,rot,interleaved", [
+    (BF, 3001, [0, 5, 40, 17], [3001, 0, 2999, 1500], 6, 64, 64, True, 64, False),
+    (HF, 5003, [3, 0], [5003, 4800], 5, 128, 24, False, 96, True),
+])
+def test_append_of_many_tokens(built_library, dtype, T, held, lengths, H, D, page, heads, rot, interleaved):
+    test_append(built_library, dtype, T, held, lengths, H, D, page, heads, rot, interleaved)
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_drawn_calls(built_library, seed):
     """Calls of all kinds: sizes, divisions of the work, page sizes, layouts, depth rows of one or several positions, own rows, rotations.  Two calls in

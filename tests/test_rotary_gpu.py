@@ -43,6 +43,13 @@ def test_forward_and_gradients(built_library, B, T, H, G, D, rot, dtype, interle
         _check(got.detach(), x.detach(), at, rotary, what, inverse)
 
 
+# more tokens than warps run at once: two or four a warp, in steps
+@pytest.mark.parametrize("B,T,H,G,D,rot", [(1, 10001, 1, 4, 64, 64), (3, 3335, 3, 3, 64, 32), (2, 4802, 4, 4, 64, 48), (1, 9999, 3, 2, 128, 128), (2, 2501, 2, 2, 128, 64)])
+@pytest.mark.parametrize("dtype,interleaved,scale", [(torch.bfloat16, False, 1.0), (torch.float16, True, 1.25)])
+def test_many_tokens_of_few_heads(built_library, B, T, H, G, D, rot, dtype, interleaved, scale):
+    test_forward_and_gradients(built_library, B, T, H, G, D, rot, dtype, interleaved, scale)
+
+
 @pytest.mark.parametrize("make", [
     lambda B, T: (None, torch.arange(T)), lambda B, T: (0, torch.arange(T)), lambda B, T: (12345, 12345 + torch.arange(T)),
     lambda B, T: (-3, torch.arange(T) - 3), lambda B, T: (torch.arange(T, dtype=torch.int32) * 3, torch.arange(T) * 3),
