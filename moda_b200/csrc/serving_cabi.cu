@@ -176,9 +176,14 @@ int divide(const moda_problem* pr, int64_t most_rows, Division* out) {
     if (units > most) break;
     log_size = next;
   }
+  // A cluster's CTAs may have up to 32 tiles each, or 52 times the part of the device that they fill if that is more: an even division
+  // fills all of it, but takes a second launch.  Rows as long as the table allows, and half of that on average, D = 128, 8 heads (128 CTAs of 296), 28 tiles:
+  // 13.2 and 11.4 us against 13.8 and 12.6, 44 tiles: 17.7 and 14.7 against 15.3 and 14.2; 32 heads (256 CTAs), 44 tiles: 19.3 and 16.5
+  // against 24.3 and 15.4; 296 heads, 49 tiles: 22.6 and 17.5 against 26.4 and 20.5
   const int cluster = 1 << log_size;
-  if (units <= slots && tiles <= 32 * cluster) {
-    *out = {(int)(units * cluster), cluster};
+  const int64_t ctas = units * cluster;
+  if (ctas <= slots && tiles * slots <= cluster * std::max(32 * slots, 52 * ctas)) {
+    *out = {(int)ctas, cluster};
     return MODA_OK;
   }
   // more units than CTAs, and none long: whole ones to warps, without a division by lengths and without parts to join.  1000 units of up

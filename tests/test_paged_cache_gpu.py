@@ -70,6 +70,11 @@ DECODE = [  # dtype, lengths, H, G, D, L, page, heads
     # more sequences than a CTA has threads, in units of single warps, of which many have none
     (BF, [(61 * i) % 198 for i in range(299)], 2, 2, 128, 1, 16, True),
     (HF, [(7 * i) % 90 for i in range(700)], 3, 1, 64, 3, 64, False),
+    # just within what clusters are given, and beyond it
+    (BF, [1530, 0, 700, 1531] * 9, 5, 2, 64, 7, 24, False),
+    (HF, [2900, 2901] * 18, 5, 4, 64, 0, 32, True),
+    (BF, [2700, 100, 2730, 5], 8, 4, 128, 16, 64, True),
+    (BF, [12000, 11999], 8, 8, 64, 11, 256, True),
 ]
 
 
