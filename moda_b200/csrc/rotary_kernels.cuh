@@ -43,15 +43,17 @@ struct Args {                // how vectors are turned
 };
 
 // Cosine and sine of position pos at frequency f, times the factor.  Whole quarter turns are taken off in integers; what is left, at
-// most an eighth of a turn (x = pi / 4), goes through the Taylor series in 64 bits (first terms left out: x^13 / 13! = 7e-12, x^12 / 12! =
-// 1.2e-10), so that the only error to speak of is the rounding to 32 bits at the end.  A lane does this once or twice a token.
+// most an eighth of a turn, becomes a number of 53 bits of its own (a slow pair's angle near the start is a small part of a turn: the
+// upper 32 bits of the fraction alone would hold 1.6e-8 radians, of base 1e7 stretched by 8, with an error of a tenth), x = pi / 4 at most,
+// which goes through the Taylor series in 64 bits (first terms left out: x^13 / 13! = 7e-12, x^12 / 12! = 1.2e-10), so that the
+// error that counts is the rounding to 32 bits at the end.  A lane does this once or twice a token.
 __device__ __forceinline__ float2 cos_sin(const Args& a, double f, long long pos) {
   constexpr double kHi = 0.15915494309189535, kLo = -9.839338337591243e-18;      // 1 / 2 pi
   const double all = f * kHi, rest = fma(f, kLo, fma(f, kHi, -all));
   const unsigned long long step = (unsigned long long)((all - floor(all)) * 18446744073709551616.0) + (unsigned long long)(long long)(rest * 18446744073709551616.0);
-  const uint32_t turn = (uint32_t)((step * (unsigned long long)pos) >> 32);        // of a turn, times 2^32
-  const uint32_t quarters = (turn + 0x20000000u) >> 30;
-  const double x = (double)(int)(turn - (quarters << 30)) * 1.4629180792671596e-9, x2 = x * x;      // 2 pi / 2^32
+  const unsigned long long turn = step * (unsigned long long)pos;                  // of a turn, times 2^64
+  const unsigned long long quarters = (turn + (1ull << 61)) >> 62;
+  const double x = (double)(long long)(turn - (quarters << 62)) * 3.4061215800865545e-19, x2 = x * x;      // 2 pi / 2^64
   double s = -1. / 39916800., c = -1. / 3628800.;
   s = fma(s, x2, 1. / 362880.);
   c = fma(c, x2, 1. / 40320.);
@@ -64,8 +66,8 @@ __device__ __forceinline__ float2 cos_sin(const Args& a, double f, long long pos
   s = fma(s * x2, x, x) * (double)a.scale;
   c = fma(c, x2, 1.) * (double)a.scale;
   float fs = (float)s, fc = (float)c;
-  if (quarters & 1u) { const float t = fc; fc = -fs; fs = t; }
-  if (quarters & 2u) { fc = -fc; fs = -fs; }
+  if (quarters & 1) { const float t = fc; fc = -fs; fs = t; }
+  if (quarters & 2) { fc = -fc; fs = -fs; }
   return make_float2(fc, a.inverse ? -fs : fs);
 }
 

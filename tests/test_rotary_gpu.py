@@ -264,3 +264,22 @@ def test_prompt_attention_with_positions(built_library):
     want = (dq.reshape(B, N, -1), torch.stack([dk, ref[4].double()], 2).reshape(B, N, -1))
     for a, b in zip(got, want):
         assert ((a.cpu().double() - b).norm() / b.norm()).item() <= 5e-2      # the attention's own tolerance for gradients
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,base,factor", [(128, 1e4, 1.0), (128, 5e5, 8.0), (64, 1e7, 8.0)])
+def test_slow_pairs_near_the_start(built_library, interleaved, D, base, factor):
+    """Pairs (0, 1) turn to (-sin a, cos a), down to a = 2.1e-8: the angle is a small part of a turn, and its sine is to have as many significant
+    digits as any other result.  bf16 rounds by half a step.  Before that, relative to the sine: the frequency in turns is cut at 2^-64
+    of a turn, 2^-35 of the smallest here (3.3e-9 turns); the series leaves out 1e-11; the sine is rounded to 32 bits (2^-24), and its product with 1 is exact."""
+    import moda_b200 as M
+    inv_freq, _ = M.rotary_frequencies(D, base, "linear", factor, device=DEV)
+    at = torch.tensor([[1, 2, 5, 33, 1000, -1]], device=DEV)
+    x = torch.zeros(1, 6, 1, D, device=DEV, dtype=torch.bfloat16)
+    first, second = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, D // 2), slice(D // 2, D))
+    x[..., second] = 1
+    y = M.rotary_embedding(x, None, M.Rotary(inv_freq, interleaved), positions=at)
+    a = at.double()[..., None, None] * inv_freq
+    for got, want in ((y[..., first], -a.sin()), (y[..., second], a.cos())):
+        # the reference rounds p f to 2^-53 of it: next to a zero of the function that is 2^-53 of a over the result
+        close(got, want, (torch.finfo(torch.bfloat16).eps / 2 * (1 + 2.0 ** -20) + 2.0 ** -23) * want.abs() + 2.0 ** -52 * a.abs(), "slow pairs")
