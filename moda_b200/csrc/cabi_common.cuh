@@ -46,6 +46,16 @@ inline View to_view(const moda_tensor4* t) {
   return v;
 }
 
+// The same of extents [B, T, H], with stride 0 where there is but one of a dimension: for kernels that also form addresses behind the last row, which
+// they do not read, but which have to be as aligned as others.
+inline View to_view(const moda_tensor4* t, int64_t B, int64_t T, int64_t H) {
+  View v = to_view(t);
+  if (B == 1) v.sb = 0;
+  if (T == 1) v.st = 0;
+  if (H == 1) v.sh = 0;
+  return v;
+}
+
 inline int cuda_fail(cudaError_t e) { g_last_cuda_error = (int)e; return MODA_ERR_CUDA; }
 
 #define MODA_CUDA(x) do { cudaError_t e__ = (x); if (e__ != cudaSuccess) return cuda_fail(e__); } while (0)

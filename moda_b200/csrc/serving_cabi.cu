@@ -43,7 +43,7 @@ int check_pages(const moda_problem* pr, const moda_paged_cache* c, paged::Pages*
   if ((reinterpret_cast<uintptr_t>(c->block_table) | reinterpret_cast<uintptr_t>(c->seq_lens)) & 3u) return MODA_ERR_ALIGNMENT;
   if (int rc = check_tensor(&c->k, true, c->num_pages, c->page_size, pr->H)) return rc;
   if (int rc = check_tensor(&c->v, true, c->num_pages, c->page_size, pr->H)) return rc;
-  out->k = to_view(&c->k); out->v = to_view(&c->v);
+  out->k = to_view(&c->k, c->num_pages, c->page_size, pr->H); out->v = to_view(&c->v, c->num_pages, c->page_size, pr->H);
   out->table = c->block_table; out->table_stride = c->table_stride; out->seq_lens = c->seq_lens;
   out->num_pages = c->num_pages; out->page_size = c->page_size; out->max_pages = c->max_pages;
   out->room = (int)std::min<int64_t>((int64_t)c->max_pages * c->page_size, 0x7fffffff);
@@ -108,7 +108,7 @@ template <typename T, int D> cudaError_t launch_append(const paged::AppendParams
 int append(const moda_problem* pr, const moda_tensor4* k, const moda_tensor4* v, const paged::Pages& pages, const int32_t* lengths,
            const rotary::Args& rot, int n_sm, cudaStream_t st) {
   paged::AppendParams p{};
-  p.k = to_view(k); p.v = to_view(v); p.pages = pages; p.lengths = lengths; p.rot = rot;
+  p.k = to_view(k, pr->B, pr->T_kv, pr->H); p.v = to_view(v, pr->B, pr->T_kv, pr->H); p.pages = pages; p.lengths = lengths; p.rot = rot;
   p.B = pr->B; p.T = pr->T_kv; p.H = pr->H; p.by_t = rotary::FastDiv((uint32_t)pr->T_kv);
   const TokenGrid grid = token_grid((int64_t)pr->B * pr->T_kv, 2 * pr->H, pr->D, n_sm);
   p.per_warp = grid.per_warp;
@@ -257,7 +257,8 @@ int moda_b200_rotary(const moda_problem* prob, const moda_rotary* rot, const mod
     if (reinterpret_cast<uintptr_t>(positions->data) & (positions->is_int64 ? 7u : 3u)) return MODA_ERR_ALIGNMENT;
     p.pos = rotary::Positions{positions->data, positions->stride_b, positions->stride_t, positions->offset, positions->is_int64 != 0};
   }
-  p.q = to_view(q); p.k = to_view(has_k ? k : nullptr); p.q_out = to_view(q_out); p.k_out = to_view(has_k ? k_out : nullptr);
+  p.q = to_view(q, B, T * prob->G, H); p.k = to_view(has_k ? k : nullptr, B, T, H);
+  p.q_out = to_view(q_out, B, T * prob->G, H); p.k_out = to_view(has_k ? k_out : nullptr, B, T, H);
   p.B = prob->B; p.T = prob->T_kv; p.H = prob->H; p.G = prob->G;
   p.vectors = prob->H * (prob->G + (has_k ? 1 : 0));
   p.by_h = rotary::FastDiv((uint32_t)prob->H); p.by_t = rotary::FastDiv((uint32_t)prob->T_kv);
@@ -340,8 +341,8 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
     if (P > 1 && (depth->k_stride_position <= 0 || depth->k_stride_position % 8 || depth->v_stride_position <= 0 || depth->v_stride_position % 8))
       return MODA_ERR_ALIGNMENT;
     if (reinterpret_cast<uintptr_t>(depth->positions_seen) & 3u) return MODA_ERR_ALIGNMENT;
-    p.kd = to_view(&depth->k); p.vd = to_view(&depth->v);
-    p.kd_sp = depth->k_stride_position; p.vd_sp = depth->v_stride_position;
+    p.kd = to_view(&depth->k, B, prob->L, H); p.vd = to_view(&depth->v, B, prob->L, H);
+    p.kd_sp = P > 1 ? depth->k_stride_position : 0; p.vd_sp = P > 1 ? depth->v_stride_position : 0;
     p.depth_positions = depth->positions_seen; p.P = (int)P; p.L = prob->L;
     p.by_L = rotary::FastDiv((uint32_t)prob->L);
   } else if (prob->L > 0) {
@@ -366,10 +367,10 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
     if (reinterpret_cast<uintptr_t>(workspace) & 255u) return MODA_ERR_ALIGNMENT;
   }
   unsigned char* ws = static_cast<unsigned char*>(workspace);
-  p.q = to_view(q); p.o = to_view(o); p.lse = lse;
+  p.q = to_view(q, B, prob->G, H); p.o = to_view(o, B, prob->G, H); p.lse = lse;
   p.B = prob->B; p.H = prob->H; p.G = prob->G; p.rows = std::min(prob->G, paged::kQ);
-  p.k = to_view(own_key ? k : nullptr); p.v = to_view(own_key ? v : nullptr);
-  p.k_copy = to_view(own_key ? k_copy : nullptr); p.v_copy = to_view(own_key ? v_copy : nullptr);
+  p.k = to_view(own_key ? k : nullptr, B, 1, H); p.v = to_view(own_key ? v : nullptr, B, 1, H);
+  p.k_copy = to_view(own_key ? k_copy : nullptr, B, 1, H); p.v_copy = to_view(own_key ? v_copy : nullptr, B, 1, H);
   p.scale_log2 = prob->scale * 1.4426950408889634f;
   p.parts = reinterpret_cast<int2*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + parts_bytes(n_cta));

@@ -642,3 +642,41 @@ def test_generating_with_a_stack_of_layers(built_library, chunk_visible, G):
         for b in range(B):
             assert torch.equal(rows_of(cache.k, table[b], T), k[b]) and torch.equal(rows_of(cache.v, table[b], T), v[b])
     assert M.device_status() == 0
+
+
+def test_any_stride_where_there_is_one_row(built_library):
+    """Pages of one row, one depth layer (of one position and of several), one head and one sequence, whose strides are not multiples of 8."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(22)
+    G, D = 3, 64
+
+    def odd(x, dim):                                                     # the same memory, stride 65 where the extent is 1
+        assert x.shape[dim] == 1
+        stride = list(x.stride())
+        stride[dim] = 65
+        return x.as_strided(x.shape, stride)
+
+    for B, H, page, L, P in ((2, 2, 1, 1, 1), (3, 2, 1, 1, 2), (1, 1, 16, 1, 1), (2, 1, 24, 1, 3), (1, 2, 1, 5, 1)):
+        lens = [19, 1, 16][:B]
+        caches, table, n = _pool(gen, BF, lens, 2, page, H, D, heads=False)
+        q, k, v = _rand(gen, BF, B, G, H, D), _rand(gen, BF, B, 1, H, D), _rand(gen, BF, B, 1, H, D)
+        depth = [_rand(gen, BF, B, P, L, H, D) for _ in range(2)]
+        seen = list(range(P, P - B, -1)) if P > 1 else None
+        given = [c for c in caches]
+        if page == 1:
+            given = [odd(c, 1) for c in given]
+        if H == 1:
+            given, q, k, v = [odd(c, 2) for c in given], odd(q, 2), odd(k, 2), odd(v, 2)
+        if B == 1:
+            q = odd(q, 0)
+        rows = [x if P > 1 else x[:, 0] for x in depth]
+        if L == 1:
+            rows = [odd(x, x.dim() - 3) for x in rows]
+        kw = dict(depth_positions=torch.tensor(seen, dtype=torch.int32, device=DEV)) if P > 1 else {}
+        o, lse = M.paged_moda_decode(q, *given, table, n, odd(k, 1), odd(v, 1), *rows, **kw, moda_group_num=G, need_lse=True)
+        _check_decode(o, lse, q, caches, table, [x + 1 for x in lens], D ** -0.5, depth if P > 1 else rows, seen=seen)
+        n += 1
+        M.paged_moda_append(odd(k, 1), odd(v, 1), *given, table, n)
+        for b, at in enumerate(lens):
+            assert torch.equal(caches[0][table[b, (at + 1) // page].long(), (at + 1) % page], k[b, 0])
+    assert M.device_status() == 0

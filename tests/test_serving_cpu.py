@@ -206,3 +206,32 @@ def test_frequencies(built_library, rot):
     for bad in (dict(rotary_dim=24), dict(rotary_dim=rot, scaling="other"), dict(rotary_dim=rot, scaling="yarn"), dict(rotary_dim=rot, factor=0.0)):
         with pytest.raises(AssertionError):
             M.rotary_frequencies(**bad)
+
+
+def test_strides_of_single_rows_stay_out_of_addresses(tmp_path):
+    """A dimension of one element may carry any stride.  The decoding kernel forms addresses of rows behind the last one (of 16 in a tile), which must be
+    aligned although they are not read: with one row a page, or one depth layer, that stride is not used."""
+    import os
+    import shutil
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "moda_b200", "csrc")
+    program = tmp_path / "views.cu"
+    program.write_text("""
+#include <cstdint>
+#include <cstdio>
+#include "cabi_common.cuh"
+int main() {
+  const moda_tensor4 t{reinterpret_cast<void*>(0x1000), 65, 67, 69};
+  const int64_t ext[5][3] = {{1, 1, 1}, {2, 1, 3}, {1, 4, 1}, {5, 4, 1}, {2, 3, 4}};
+  for (const auto& e : ext) {
+    const moda::View v = moda::to_view(&t, e[0], e[1], e[2]);
+    std::printf("%d %d %d\\n", (int)v.sb, (int)v.st, (int)v.sh);
+  }
+  return moda::to_view(nullptr, 1, 1, 1).ptr != nullptr;
+}
+""")
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", csrc, str(program), "-o", str(tmp_path / "views")], check=True)
+    out = subprocess.run([str(tmp_path / "views")], check=True, capture_output=True, text=True).stdout
+    assert out.splitlines() == ["0 0 0", "65 0 69", "0 67 0", "65 67 0", "65 67 69"]
