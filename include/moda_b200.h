@@ -239,6 +239,8 @@ typedef struct moda_paged_cache {
   int64_t table_stride;
   int32_t max_pages;
   const int32_t *seq_lens;    /* DEVICE [B]: rows that the sequences hold before the call                 */
+  int32_t copy_all;           /* moda_b200_paged_decode: non-zero writes k_copy, v_copy also for tokens whose
+                                 row has no place in the cache (0 leaves them as they are there)          */
 } moda_paged_cache;
 
 /* Depth rows of the new tokens.  [B, L, H, D], the rows of a token's own position (positions_per_sequence = 1);
@@ -279,7 +281,8 @@ int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, cons
  * (the key turned) to k_copy, v_copy [B, 1, H, D] as well: a layer's slot of a depth cache.  With rot, q and k are
  * turned: at position seq_lens[b] with k, v, and otherwise at seq_lens[b] - 1, that of the sequence's last row.
  * Rows in pages that are none of the pool's are left out and recorded, as are lengths that are negative or
- * more than the table covers.  Nothing that the call writes may be among the rows that it reads.
+ * more than the table covers; the token's own row too, which is then not copied either unless cache->copy_all is set: a copy
+ * that is the next layer's depth row is read there whether the row has a place here or not.  Nothing that the call writes may be among the rows that it reads.
  * The results do not depend on scheduling.  workspace: caller-owned DEVICE scratch, 256-byte aligned,
  * contents undefined on entry and exit; calls that may overlap on the GPU need one each.  How many bytes (0: none, and
  * workspace may be NULL) depends on the device, on B, H, G, D, L and on how long the table lets a sequence be (max_pages, page_size).

@@ -88,7 +88,7 @@ class Positions(ctypes.Structure):         # moda_positions
 class PagedCache(ctypes.Structure):        # moda_paged_cache
     _fields_ = [("k", Tensor4), ("v", Tensor4), ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
                 ("block_table", ctypes.c_void_p), ("table_stride", ctypes.c_int64), ("max_pages", ctypes.c_int32),
-                ("seq_lens", ctypes.c_void_p)]
+                ("seq_lens", ctypes.c_void_p), ("copy_all", ctypes.c_int32)]
 
 
 class DepthRows(ctypes.Structure):         # moda_depth_rows

@@ -48,6 +48,7 @@ struct DecodeParams {
   Pages pages;
   View k, v;                       // [B, 1, H, D]: the new tokens' own rows, which this call writes to the cache (pointers nullptr: none)
   View k_copy, v_copy;             // [B, 1, H, D]: those rows as written once more (pointers nullptr: not)
+  int copy_all;                    // also of rows that have no place in the cache (0 without the copies)
   View kd, vd;                     // depth rows (b, layer, h); position p of P lies p * depth_sp further
   int64_t kd_sp, vd_sp;
   const int* depth_positions;      // [B]: positions seen, nullptr: all P
@@ -284,7 +285,8 @@ __device__ __forceinline__ bool locate_units(const DecodeParams& p, int units, W
 }
 
 // The new token's own row, row n of a tile that has been copied as it was given: turned there, and written to its place in the cache (page, and slot
-// in it) and to the copies.  cs: cosines and sines of its position, which is the queries'.
+// in it) and to the copies.  cs: cosines and sines of its position, which is the queries'.  page < 0: it has no place, and is not seen either: its value
+// must not meet the products, where an infinite one would count times 0.
 template <typename T, int D>
 __device__ __forceinline__ void own_row(const DecodeParams& p, const Walk& w, int h, int page, bool write, uint32_t tile, int n, const float2* cs) {
   constexpr int C = D / 16;
@@ -303,11 +305,17 @@ __device__ __forceinline__ void own_row(const DecodeParams& p, const Walk& w, in
       sts128(row + ((c0 ^ swizzle) << 4), x);
       sts128(row + ((c1 ^ swizzle) << 4), y);
     }
-    if (write) {
+    if (page < 0) {
+      sts128(row + ((c0 ^ swizzle) << 4), make_uint4(0, 0, 0, 0));
+      sts128(row + ((c1 ^ swizzle) << 4), make_uint4(0, 0, 0, 0));
+    }
+    if (write && (page >= 0 || p.copy_all != 0)) {
       const int slot = w.s.held - (int)p.pages.by_page.div((uint32_t)w.s.held) * p.pages.page_size;
       const View &to = of_v ? p.pages.v : p.pages.k, &copy = of_v ? p.v_copy : p.k_copy;
-      *rotary::chunk_at(to, to.off(page, slot, h), c0) = x;
-      *rotary::chunk_at(to, to.off(page, slot, h), c1) = y;
+      if (page >= 0) {
+        *rotary::chunk_at(to, to.off(page, slot, h), c0) = x;
+        *rotary::chunk_at(to, to.off(page, slot, h), c1) = y;
+      }
       if (copy.ptr != nullptr) {
         *rotary::chunk_at(copy, copy.off(w.b, 0, h), c0) = x;
         *rotary::chunk_at(copy, copy.off(w.b, 0, h), c1) = y;
@@ -315,6 +323,26 @@ __device__ __forceinline__ void own_row(const DecodeParams& p, const Walk& w, in
     }
   }
   __syncwarp();
+}
+
+// The own row of a sequence that has no room for it (or whose length is wrong), which is in no tile: into the copies alone.  By one thread; rare.
+template <typename T, int D>
+__device__ __noinline__ void copy_own_row(const DecodeParams& p, int b, int h, int position) {
+#pragma unroll 1
+  for (int i = 0; i < 2 * (D / 16); ++i) {
+    const bool of_v = i >= D / 16;
+    int c0, c1;
+    const bool turns = rotary::item_chunks(p.rot, i % (D / 16), c0, c1) && p.rot.inv_freq != nullptr && !of_v;
+    const View &from = of_v ? p.v : p.k, &to = of_v ? p.v_copy : p.k_copy;
+    uint4 x = *rotary::chunk_at(from, from.off(b, 0, h), c0), y = *rotary::chunk_at(from, from.off(b, 0, h), c1);
+    if (turns) {
+      float2 cs[8];
+      for (int e = 0; e < 8; ++e) cs[e] = rotary::cos_sin(p.rot, p.rot.inv_freq[8 * i + e], position);
+      rotary::turn<T>(x, y, cs, p.rot.interleaved != 0);
+    }
+    *rotary::chunk_at(to, to.off(b, 0, h), c0) = x;
+    *rotary::chunk_at(to, to.off(b, 0, h), c1) = y;
+  }
 }
 
 // Copies a tile's rows one by one: where a page ends in it, where a page is missing, and where the token's own row is.  Lane l finds the K row
@@ -327,7 +355,7 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
   const bool of_v = lane >= 16;
   const unsigned char* row = static_cast<const unsigned char*>(p.pages.k.ptr);
   int page = -1;
-  bool valid, own = false;
+  bool valid, own = false;           // seen; the token's own, which is copied also where it has no page
   if (tile < s.cached_tiles) {
     const int key = tile * kTile + (lane & 15);
     valid = key < s.len;
@@ -338,10 +366,12 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
       else page = which == (int)p.pages.by_page.div((uint32_t)(tile * kTile)) ? page0 : page1;
       const int slot_of = key - which * p.pages.page_size;
       valid = page >= 0 && page < p.pages.num_pages;
-      own = own && valid;
-      if (!valid) wrong(kBadPage);
-      else if (own) row = of_v ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h) : static_cast<const unsigned char*>(p.k.ptr) + 2 * p.k.off(w.b, 0, h);
-      else row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
+      if (!valid) {
+        wrong(kBadPage);
+        page = -1;
+      }
+      if (own) row = of_v ? static_cast<const unsigned char*>(p.v.ptr) + 2 * p.v.off(w.b, 0, h) : static_cast<const unsigned char*>(p.k.ptr) + 2 * p.k.off(w.b, 0, h);
+      else if (valid) row = of_v ? static_cast<const unsigned char*>(p.pages.v.ptr) + 2 * p.pages.v.off(page, slot_of, h) : row + 2 * p.pages.k.off(page, slot_of, h);
     }
   } else {
     const int d = (tile - s.cached_tiles) * kTile + (lane & 15), pos = (int)p.by_L.div((uint32_t)d), layer = d - pos * p.L;
@@ -349,8 +379,8 @@ __device__ __forceinline__ void mixed_tile(const DecodeParams& p, const Walk& w,
     if (valid) row = of_v ? static_cast<const unsigned char*>(p.vd.ptr) + 2 * (p.vd.off(w.b, layer, h) + pos * p.vd_sp)
                           : static_cast<const unsigned char*>(p.kd.ptr) + 2 * (p.kd.off(w.b, layer, h) + pos * p.kd_sp);
   }
-  const uint32_t there = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own) & 0xffffu;
-  if (its_own == 0 ? lane == 0 : lane == __ffs(its_own) - 1) *mask = make_uint2(there | (uint32_t)__ffs(its_own) << 16, page);
+  const uint32_t seen = __ballot_sync(0xffffffffu, valid) & 0xffffu, its_own = __ballot_sync(0xffffffffu, own) & 0xffffu, there = seen | its_own;
+  if (its_own == 0 ? lane == 0 : lane == __ffs(its_own) - 1) *mask = make_uint2(seen | (uint32_t)__ffs(its_own) << 16, page);
   const unsigned long long at = reinterpret_cast<unsigned long long>(row);
 #pragma unroll 2
   for (int i = 0; i < kCopies; ++i) {
@@ -711,6 +741,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D>()) decode_kernel(cons
             for (int e = 0; e < 4; ++e) split<T>(y[2 * e], y[2 * e + 1], qh[j][e], ql[j][e]);
           }
         }
+        // the part that ends the unit has its last tile, which may not be empty: there is one such part
+        if (__builtin_expect(p.copy_all != 0 && w.s.len == w.s.held && w.t1 == w.s.tiles && w.t0 < w.t1 && q0 == 0 && rank == 0 && lane == 0, 0))
+          copy_own_row<T, D>(p, w.b, h, w.s.held);
         m = -INFINITY; l = 0.f;
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;

@@ -371,6 +371,7 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   p.B = prob->B; p.H = prob->H; p.G = prob->G; p.rows = std::min(prob->G, paged::kQ);
   p.k = to_view(own_key ? k : nullptr, B, 1, H); p.v = to_view(own_key ? v : nullptr, B, 1, H);
   p.k_copy = to_view(own_key ? k_copy : nullptr, B, 1, H); p.v_copy = to_view(own_key ? v_copy : nullptr, B, 1, H);
+  p.copy_all = p.k_copy.ptr != nullptr && cache->copy_all != 0;
   p.scale_log2 = prob->scale * 1.4426950408889634f;
   p.parts = reinterpret_cast<int2*>(ws);
   p.ml = reinterpret_cast<float2*>(ws + parts_bytes(n_cta));

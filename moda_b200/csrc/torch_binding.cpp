@@ -770,10 +770,10 @@ PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale, G, rotary, record_k, record_v) -> (o, lse)
+// paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale, G, rotary, record_k, record_v, record_all) -> (o, lse)
 PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (!arg_count(n, 15)) return nullptr;
+  if (!arg_count(n, 16)) return nullptr;
   require_type(THPVariable_Check(a[0]), "moda_b200: the operands must be tensors");
   for (int i : {5, 6, 7, 8, 9, 13, 14}) require_type(tensor_or_none_check(a[i]), "moda_b200: the operands must be tensors");
   const Tensor q_ = tensor_or_none(a[0]), k_ = tensor_or_none(a[5]), v_ = tensor_or_none(a[6]), rk = tensor_or_none(a[13]), rv = tensor_or_none(a[14]);
@@ -783,7 +783,10 @@ PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   require(q_.dim() == 4 && G > 0 && q_.size(1) == G, "q must be [B, moda_group_num, H, D]: one token of each sequence");
   const int64_t B = q_.size(0), H = q_.size(2), D = q_.size(3);
   const double scale = as_scale(a[10], q_);
-  const PagedCache c = as_paged(a + 1, B, H, D);
+  PagedCache c = as_paged(a + 1, B, H, D);
+  const int record_all = PyObject_IsTrue(a[15]);
+  if (record_all < 0) throw python_error();
+  c.abi.copy_all = record_all;
   auto one_row = [&](const Tensor& x) { return x.dim() == 4 && x.size(0) == B && x.size(1) == 1 && x.size(2) == H && x.size(3) == D; };
   require(k_.defined() == v_.defined(), "k and v must be given together");
   require(!k_.defined() || (one_row(k_) && one_row(v_)), "k and v must be [B, 1, H, D]");

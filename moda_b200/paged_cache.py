@@ -45,7 +45,7 @@ def paged_moda_decode(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Ten
                       cached_k: Optional[torch.Tensor] = None, cached_v: Optional[torch.Tensor] = None,
                       depth_positions: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                       moda_group_num: int = 1, rotary: Optional[Rotary] = None, need_lse: bool = False,
-                      record_k: Optional[torch.Tensor] = None, record_v: Optional[torch.Tensor] = None):
+                      record_k: Optional[torch.Tensor] = None, record_v: Optional[torch.Tensor] = None, record_all: bool = False):
     """MoDA attention of one new token of each sequence: ``q [B, G, H, D]`` -> ``o [B, G, H, D]``, or ``(o, lse)`` with ``lse``
     fp32 ``[B, G, H]`` in base-2 units.
 
@@ -54,9 +54,10 @@ def paged_moda_decode(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Ten
     ``cached_k, cached_v``: ``[B, L, H, D]`` of its own position, or ``[B, P, L, H, D]`` of positions of its chunk, of which it sees the
     first ``depth_positions[b]`` (int32; chunk-visible).  With ``rotary`` ``q`` and ``k`` are turned at the token's position;
     depth rows are used as they are.  ``record_k, record_v [B, 1, H, D]`` (none of the rows that are read) receive the token's row as
-    written to the cache.  A token that sees nothing gets ``o = 0``, ``lse = -inf``."""
+    written to the cache; a token whose row has no place there leaves them as they are, unless ``record_all``.  A token that sees
+    nothing gets ``o = 0``, ``lse = -inf``."""
     r = _cabi.native().paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale,
-                                    moda_group_num, rotary, record_k, record_v)
+                                    moda_group_num, rotary, record_k, record_v, record_all)
     return r if need_lse else r[0]
 
 
@@ -78,7 +79,8 @@ class PagedKVCache:
                record: bool = False, scale=None, moda_group_num: int = 1, rotary=None, need_lse: bool = False):
         """``paged_moda_decode`` over this layer's pages and the layers that ``depth`` holds: a cache of one position, or (with
         ``depth_positions``) of the positions of a chunk.  ``record``: the token's row also becomes the next layer of ``depth``
-        (of one position), for the layers after this one."""
+        (of one position), for the layers after this one: also where it has no place in the pages, which leaves it out of this layer
+        alone."""
         cached_k = cached_v = record_k = record_v = None
         if depth is not None:
             ck, cv = (x.view(depth.B, depth.T, depth.capacity, depth.H, depth.D) for x in (depth.k, depth.v))
@@ -92,7 +94,7 @@ class PagedKVCache:
             assert depth.L < depth.capacity, "DepthKVCache is full"
             record_k, record_v = ck[:, :, depth.L], cv[:, :, depth.L]
         r = paged_moda_decode(q, self.k, self.v, block_table, seq_lens, k, v, cached_k, cached_v,
-                              depth_positions if cached_k is not None else None, scale, moda_group_num, rotary, need_lse, record_k, record_v)
+                              depth_positions if cached_k is not None else None, scale, moda_group_num, rotary, need_lse, record_k, record_v, record)
         if record:
             depth.L += 1
         return r

@@ -680,3 +680,69 @@ def test_any_stride_where_there_is_one_row(built_library):
         for b, at in enumerate(lens):
             assert torch.equal(caches[0][table[b, (at + 1) // page].long(), (at + 1) % page], k[b, 0])
     assert M.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype,B,G,D,page,pages_each,long", [
+    (BF, 3, 9, 64, 16, 20, 300),            # a unit to a cluster
+    (HF, 4, 2, 128, 16, 2, 32),             # to a CTA
+    (HF, 8, 4, 128, 16, 1200, 9600),        # divided evenly
+    (BF, 900, 3, 64, 16, 3, 48),            # whole units to warps
+    (HF, 700, 2, 128, 16, 40, 60),          # divided evenly, short units to warps
+])
+@pytest.mark.parametrize("turned", [False, True])
+def test_the_next_layer_sees_a_row_without_a_place(built_library, dtype, B, G, D, page, pages_each, long, turned):
+    """Two layers over a depth cache that holds NaN: sequences whose row the table has no room for, whose page is none of the pool's, or whose length is
+    negative.  The first layer leaves the row out; it is the second layer's depth row all the same, turned at the position that the query takes."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(23)
+    H = 2
+    room = pages_each * page
+    table = torch.randperm(B * pages_each, generator=gen, device=DEV).view(B, pages_each).int()
+    lens = [min(long, room - 1) - (7 * b) % 30 for b in range(B)]
+    broken = {0: "no room", B // 2: "bad page", B - 1: "negative"}
+    lens[0], lens[B // 2] = room, 33 if room > 33 else 17
+    table[B // 2, lens[B // 2] // page] = -1 if B % 2 else B * pages_each
+    held = [0 if broken.get(b) == "negative" else x for b, x in enumerate(lens)]
+    n = torch.tensor([-5 if broken.get(b) == "negative" else x for b, x in enumerate(lens)], dtype=torch.int32, device=DEV)
+    at = torch.tensor(held, device=DEV)
+    rotary = M.Rotary(M.rotary_frequencies(D, device=DEV)[0], True, 1.1) if turned else None
+    layers = [M.PagedKVCache(B * pages_each, page, H, D, dtype, DEV) for _ in range(2)]
+    depth = M.DepthKVCache(B, 1, 3, H, D, dtype, DEV)
+    for x in (depth.k, depth.v):
+        x.fill_(float("nan"))
+    rows = []
+    for i, layer in enumerate(layers):
+        for x in (layer.k, layer.v):
+            x.copy_(torch.randn(x.shape, generator=gen, device=DEV))
+        q, k, v = _rand(gen, dtype, B, G, H, D), _rand(gen, dtype, B, 1, H, D), _rand(gen, dtype, B, 1, H, D)
+        before = [layer.k.clone(), layer.v.clone()]
+        o, lse = layer.decode(q, table, n, k, v, depth=depth, record=True, moda_group_num=G, rotary=rotary, need_lse=True)
+        assert M.device_status() in ((2 << 8 | 1), (2 << 8 | 2)) and M.device_status() == 0 and depth.L == i + 1
+        for b, why in broken.items():
+            keys, values = (rows_of(c, table[b].clamp(0, B * pages_each - 1), held[b]).double() for c in (layer.k, layer.v))
+            if why == "bad page":
+                first = held[b] // page * page
+                keys, values = keys[:first], values[:first]
+            if i:
+                keys, values = torch.cat([keys, rows[0][b].double()]), torch.cat([values, rows[1][b].double()])
+            q64 = turn(q[b : b + 1].double(), at[b : b + 1, None], rotary.inv_freq, True, 1.1)[0] if turned else q[b].double()
+            want = attend(q64, keys, values, D ** -0.5)
+            tol = attend_bounds(*want, D, dtype, turned)
+            close(o[b], want[0], tol[0], why), close(lse[b], want[1], tol[1], why)
+        others = [b for b in range(B) if b not in broken][:40]
+        _check_decode(o[others], lse[others], q[others], (layer.k, layer.v), table[others], [lens[b] + 1 for b in others], D ** -0.5,
+                      [x[others] for x in rows] if i else None, (rotary, at[others]) if turned else None)
+        rows = [x.view(B, 3, H, D)[:, i : i + 1].clone() for x in (depth.k, depth.v)]
+        want_k = turn(k.double(), at[:, None], rotary.inv_freq, True, 1.1) if turned else k.double()
+        close(rows[0], want_k, turn_bound(k.double(), want_k, D, True, 1.1, dtype) if turned else torch.zeros_like(want_k), "recorded keys")
+        assert torch.equal(rows[1], v)
+        ok = torch.tensor([b for b in range(B) if b not in broken], dtype=torch.long, device=DEV)
+        pages, slots = table[ok, at[ok] // page].long(), at[ok] % page
+        for c, old, new in zip((layer.k, layer.v), before, rows):        # nothing else has been written
+            old[pages, slots] = new[ok, 0]
+            assert torch.equal(c, old)
+    if not turned:                                                       # an infinite value of a row that is left out counts nowhere
+        v[:] = float("inf")
+        want = layer.decode(q, table, n, k, torch.zeros_like(v), depth=depth, moda_group_num=G)[list(broken)]
+        assert torch.equal(layer.decode(q, table, n, k, v, depth=depth, moda_group_num=G)[list(broken)], want)
+        assert M.device_status() != 0
