@@ -816,7 +816,7 @@ PyObject* py_paged_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Out r;
   {
     NoGil no_gil;
-    refuse_gradients({&q_, &k_, &v_, &c.k, &c.v, &ck_, &cv_});
+    refuse_gradients({&q_, &k_, &v_, &c.k, &c.v, &ck_, &cv_, &rk, &rv});
     at::AutoGradMode no_grad(false);
     const Tensor q = in_place_or_copy(q_), k = in_place_or_copy(k_), v = in_place_or_copy(v_), ck = in_place_or_copy(ck_), cv = in_place_or_copy(cv_);
     moda_problem pr = serving_problem(q, 1, G, scale);

@@ -746,3 +746,22 @@ def test_the_next_layer_sees_a_row_without_a_place(built_library, dtype, B, G, D
         want = layer.decode(q, table, n, k, torch.zeros_like(v), depth=depth, moda_group_num=G)[list(broken)]
         assert torch.equal(layer.decode(q, table, n, k, v, depth=depth, moda_group_num=G)[list(broken)], want)
         assert M.device_status() != 0
+
+
+@pytest.mark.parametrize("which", ["record_k", "record_v", "both", "views of a leaf"])
+def test_records_that_require_gradients_are_refused(built_library, which):
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(24)
+    caches, table, n = _pool(gen, BF, [5], 3, 8, 2, 64, fill=0.0)
+    q, k = _rand(gen, BF, 1, 1, 2, 64), _rand(gen, BF, 1, 1, 2, 64)
+    before = [c.clone() for c in caches]
+    leaf = torch.zeros(2, 1, 1, 2, 64, device=DEV, dtype=BF)
+    rk, rv = (leaf.requires_grad_()[0], leaf[1]) if which == "views of a leaf" else (leaf[0].clone(), leaf[1].clone())
+    if which != "views of a leaf":
+        rk.requires_grad_(which != "record_v"), rv.requires_grad_(which != "record_k")
+    with pytest.raises(RuntimeError, match="does not train"):
+        M.paged_moda_decode(q, *caches, table, n, k, k, record_k=rk, record_v=rv)
+    assert not rk.any() and not rv.any() and all(torch.equal(a, b) for a, b in zip(caches, before))
+    with torch.no_grad():
+        M.paged_moda_decode(q, *caches, table, n, k, k, record_k=rk, record_v=rv)
+    assert torch.equal(rk, k) and torch.equal(rv, k)
