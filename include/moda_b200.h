@@ -267,7 +267,8 @@ int moda_b200_rotary(const moda_problem *prob, const moda_rotary *rot, const mod
  * seq_lens[b] + t, for t < lengths[b] (DEVICE [B]; NULL: all T_kv).  Keys are turned on the way when rot
  * is not NULL, at the position that is their row.  seq_lens stays as it is.  Rows that are to be written must
  * lie in pages of one sequence only.  A token whose page is none of the pool's, or whose row the table does not
- * cover, is left out and recorded (moda_b200_device_status).
+ * cover, is left out and recorded (moda_b200_device_status).  So is a lengths[b] that is negative (none of the tokens
+ * are written) or more than T_kv (all of them are).
  */
 int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, const moda_tensor4 *v,
                            const moda_paged_cache *cache, const int32_t *lengths, const moda_rotary *rot,
@@ -329,7 +330,7 @@ const char *moda_b200_kernel_name(int kernel_id);
  * wants to know that its results are valid reads it at its next synchronisation point
  * (0 = every launch since the previous read ran to completion).  The paged-cache calls
  * record here what they left out: (2 << 8 | 1) a page that is none of the pool's, (2 << 8 | 2) a
- * length that is negative or more than the table covers; where both kinds were recorded the next call
+ * length that is negative or more than the table covers (or than the tokens of an append); where both kinds were recorded the next call
  * returns the second.  SYNCHRONISES the device.  The reference has no counterpart (Triton kernels do not spin on barriers
  * they could miss).
  */

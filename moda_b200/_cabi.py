@@ -223,7 +223,8 @@ def device_status() -> int:
     0 = every launch since the previous read ran to completion.  Non-zero = the first wait that
     expired since then ((1 << 8) | barrier id): that launch returned early and left outputs
     unwritten; or what a paged-cache call left out first ((2 << 8) | 1: a page that is none of the
-    pool's, (2 << 8) | 2: a length that is negative or more than the table covers).  Reading resets the word, so callers poll it at their next synchronisation point."""
+    pool's, (2 << 8) | 2: a length that is negative or more than the table covers, or than an append has tokens).
+    Reading resets the word, so callers poll it at their next synchronisation point."""
     v = ctypes.c_int(0)
     check(load().moda_b200_device_status(ctypes.byref(v)), "moda_b200_device_status")
     return int(v.value)

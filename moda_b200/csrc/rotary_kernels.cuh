@@ -237,7 +237,11 @@ __global__ void __launch_bounds__(rotary::kThreads, rotary::kBlocks) append_kern
   const int64_t tok = ((int64_t)blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * kTokens + lane / (C * kLanes);
   bool active = tok < (int64_t)p.B * p.T;
   const int b = active ? (int)p.by_t.div((uint32_t)tok) : 0, t = active ? (int)(tok - (int64_t)b * p.T) : 0;
-  active = active && (p.lengths == nullptr || t < p.lengths[b]);
+  if (active && p.lengths != nullptr) {
+    const int given = p.lengths[b];
+    if (given < 0 || given > p.T) wrong(kBadLength);
+    active = t < given;
+  }
   if (!__any_sync(0xffffffffu, active)) return;
   float2 cs[8];
   int page = 0, slot = 0;

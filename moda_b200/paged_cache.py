@@ -36,7 +36,8 @@ def paged_moda_append(k: torch.Tensor, v: torch.Tensor, cache_k: torch.Tensor, c
 
     Token ``t`` of sequence ``b`` becomes row ``seq_lens[b] + t``, for ``t < lengths[b]`` (None: all of them).  With
     ``rotary`` keys are turned on the way, at their row's position.  ``block_table`` int32 ``[B, max_pages]``; ``seq_lens``,
-    ``lengths`` int32 ``[B]``; ``seq_lens`` is not changed.  A page that is written to must belong to one sequence."""
+    ``lengths`` int32 ``[B]``; ``seq_lens`` is not changed.  A ``lengths[b]`` below 0 or above ``T`` counts as 0 or
+    ``T`` and is recorded (``device_status()``).  A page that is written to must belong to one sequence."""
     _cabi.native().paged_append(k, v, cache_k, cache_v, block_table, seq_lens, lengths, rotary)
 
 

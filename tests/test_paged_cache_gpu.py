@@ -765,3 +765,25 @@ def test_records_that_require_gradients_are_refused(built_library, which):
     with torch.no_grad():
         M.paged_moda_decode(q, *caches, table, n, k, k, record_k=rk, record_v=rv)
     assert torch.equal(rk, k) and torch.equal(rv, k)
+
+
+@pytest.mark.parametrize("H,D,T", [(2, 64, 3), (20, 128, 5), (1, 64, 40)])
+@pytest.mark.parametrize("bad", [-1, -(2 ** 31), "T + 1", 2 ** 31 - 1])
+def test_append_of_more_tokens_than_there_are(built_library, H, D, T, bad):
+    """A length of the call that is negative or more than T is recorded; what there is is written, and no more."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(25)
+    bad = T + 1 if bad == "T + 1" else bad
+    held, page = [7, 0, 16], 8
+    caches, table, n = _pool(gen, BF, held, T + 3, page, H, D)
+    before = [c.clone() for c in caches]
+    k, v = _rand(gen, BF, 3, T, H, D), _rand(gen, BF, 3, T, H, D)
+    M.paged_moda_append(k, v, *caches, table, n, torch.tensor([T, 0, 1], dtype=torch.int32, device=DEV))
+    assert M.device_status() == 0
+    M.paged_moda_append(k, v, *caches, table, n, torch.tensor([T, bad, 1], dtype=torch.int32, device=DEV))
+    assert M.device_status() == (2 << 8 | 2) and M.device_status() == 0
+    for b, count in enumerate([T, 0 if bad < 0 else T, 1]):
+        at = held[b] + torch.arange(count, device=DEV)
+        for old, x in zip(before, (k, v)):
+            old[table[b, at // page].long(), at % page] = x[b, :count]
+    assert all(torch.equal(c.view(torch.int16), old.view(torch.int16)) for c, old in zip(caches, before))
