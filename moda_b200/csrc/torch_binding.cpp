@@ -328,7 +328,9 @@ RotarySpec as_rotary(PyObject* x, const Tensor& like) {
   RotarySpec r;
   require_type(PyTuple_Check(x) && PyTuple_GET_SIZE(x) == 3 && THPVariable_Check(PyTuple_GET_ITEM(x, 0)), "moda_b200: rotary must be a moda_b200.Rotary");
   r.inv_freq = THPVariable_Unpack(PyTuple_GET_ITEM(x, 0));
-  r.interleaved = PyObject_IsTrue(PyTuple_GET_ITEM(x, 1)) == 1;
+  const int interleaved = PyObject_IsTrue(PyTuple_GET_ITEM(x, 1));
+  if (interleaved < 0) throw python_error();
+  r.interleaved = interleaved == 1;
   r.scale = PyFloat_AsDouble(PyTuple_GET_ITEM(x, 2));
   if (r.scale == -1. && PyErr_Occurred()) throw python_error();
   require_type(r.inv_freq.scalar_type() == at::kDouble, "moda_b200: inv_freq must be float64");

@@ -235,3 +235,21 @@ int main() {
     subprocess.run([nvcc, "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a", "-I", csrc, str(program), "-o", str(tmp_path / "views")], check=True)
     out = subprocess.run([str(tmp_path / "views")], check=True, capture_output=True, text=True).stdout
     assert out.splitlines() == ["0 0 0", "65 0 69", "0 67 0", "65 67 0", "65 67 69"]
+
+
+def test_what_interleaved_raises_is_not_lost(built_library):
+    import moda_b200 as M
+    q = torch.zeros(2, 4, 2, 64, dtype=BF)
+
+    class Bad:
+        def __bool__(self):
+            raise ValueError("no truth in it")
+
+    for bad, error, match in ((torch.zeros(2), RuntimeError, "ambiguous"), (Bad(), ValueError, "no truth in it")):
+        rotary = _rotary(M, interleaved=bad)
+        with pytest.raises(error, match=match):
+            M.rotary_embedding(q, None, rotary)
+        with pytest.raises(error, match=match):
+            M.paged_moda_append(q, q, rotary=rotary, **_paged())
+        with pytest.raises(error, match=match):
+            M.paged_moda_decode(q, moda_group_num=4, rotary=rotary, **_paged())
