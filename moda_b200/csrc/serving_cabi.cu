@@ -160,6 +160,11 @@ template <int D> int clusters_at_once(int device, int log_size, int* out) {
   return MODA_OK;
 }
 
+// The decoding kernels count keys, and the tiles of one head of all sequences, in 31 bits.
+bool too_many_keys(int64_t B, int64_t most_keys) {
+  return most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 2 + paged::unit_cost(paged::kWarps)) > 0x7fffffff;
+}
+
 // How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
 // the width of its table (and L depth rows).
 struct Division { int ctas, cluster; };
@@ -304,6 +309,7 @@ int moda_b200_paged_decode_workspace_bytes(const moda_problem* prob, const moda_
   if (bytes == nullptr || cache == nullptr) return MODA_ERR_NULL;
   if (int rc = check_sizes(prob)) return rc;
   if (cache->max_pages < 1 || cache->page_size < 1) return MODA_ERR_SHAPE;
+  if (too_many_keys(prob->B, (int64_t)cache->max_pages * cache->page_size)) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
   Division div;
@@ -350,9 +356,7 @@ int moda_b200_paged_decode(const moda_problem* prob, const moda_tensor4* q, cons
   } else {
     p.kd = p.vd = View{p.pages.k.ptr, 0, 0, 0};      // no row of it is read
   }
-  // the kernels count keys, and the tiles of one head of all sequences, in 31 bits
-  const int64_t most_keys = (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L;
-  if (most_keys > 0x7fffffff - 64 || B * (most_keys / paged::kTile + 2 + paged::unit_cost(paged::kWarps)) > 0x7fffffff) return MODA_ERR_TOO_LARGE;
+  if (too_many_keys(B, (int64_t)p.pages.max_pages * p.pages.page_size + own_key + (int64_t)p.P * p.L)) return MODA_ERR_TOO_LARGE;
   DeviceGuard guard(prob->device);
   if (!guard.ok) return cuda_fail(guard.err);
   Division div;

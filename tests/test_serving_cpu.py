@@ -253,3 +253,19 @@ def test_what_interleaved_raises_is_not_lost(built_library):
             M.paged_moda_append(q, q, rotary=rotary, **_paged())
         with pytest.raises(error, match=match):
             M.paged_moda_decode(q, moda_group_num=4, rotary=rotary, **_paged())
+
+
+def test_workspace_of_tables_too_large(built_library):
+    """What the attention itself refuses has no workspace either (2^62 rows would not fit the division's numbers)."""
+    from moda_b200 import _cabi
+    from moda_b200._cabi import PagedCache, Problem, Tensor4
+    lib, big = _cabi.load(), 2 ** 31 - 1
+    t = Tensor4(0x1000, 1024, 256, 64)
+    n = ctypes.c_size_t(7)
+    for B, pages, page in ((1, big, big), (1, big, 2), (1, 1, big), (65535, 1 << 20, 1)):
+        prob = Problem(B=B, T_kv=1, H=2, D=64, G=2, L=0, dtype=0, scale=0.125, device=0)
+        cache = PagedCache(k=t, v=t, num_pages=4, page_size=page, block_table=0x2000, table_stride=2, max_pages=pages, seq_lens=0x3000)
+        r = ctypes.byref
+        assert lib.moda_b200_paged_decode_workspace_bytes(r(prob), r(cache), r(n)) == 11
+        assert lib.moda_b200_paged_decode(r(prob), r(t), r(cache), None, None, None, None, None, None, r(t), 0x4000, 0x8000, 0, None) == 11
+    assert n.value == 7
