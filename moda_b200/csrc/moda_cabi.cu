@@ -506,6 +506,7 @@ const char* moda_b200_kernel_name(int kernel_id) { return prof::kernel_name(kern
 
 int moda_b200_device_status(int* status) {
   if (status == nullptr) return MODA_ERR_NULL;
+  MODA_CUDA(cudaDeviceSynchronize());      // the copies below wait for streams that wait for the default stream alone
   int v = 0;
   const int e = tc::read_status(&v);
   if (e != 0) { g_last_cuda_error = e; return MODA_ERR_CUDA; }

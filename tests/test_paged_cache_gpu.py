@@ -787,3 +787,23 @@ def test_append_of_more_tokens_than_there_are(built_library, H, D, T, bad):
         for old, x in zip(before, (k, v)):
             old[table[b, at // page].long(), at % page] = x[b, :count]
     assert all(torch.equal(c.view(torch.int16), old.view(torch.int16)) for c, old in zip(caches, before))
+
+
+def test_status_waits_for_streams_of_any_kind(built_library):
+    """A stream that does not wait for the default one, with work in front of the call that leaves something out."""
+    import moda_b200 as M
+    gen = torch.Generator(device=DEV).manual_seed(26)
+    caches, table, n = _pool(gen, BF, [5], 3, 8, 2, 64)
+    k = _rand(gen, BF, 1, 1, 2, 64)
+    broken = table.clone()
+    broken[0, 0] = -1
+    a = torch.randn(8192, 8192, device=DEV, dtype=BF)
+    side = torch.cuda.Stream()
+    for t, times in ((table, 1), (broken, 60)):          # a first launch may wait for the device by itself
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for _ in range(times):
+                b = a @ a
+            M.paged_moda_append(k, k, *caches, t, n)
+        assert M.device_status() == (0 if t is table else 2 << 8 | 1) and M.device_status() == 0
+    assert side.query() and b.shape == a.shape
