@@ -280,7 +280,8 @@ int moda_b200_paged_append(const moda_problem *prob, const moda_tensor4 *k, cons
  * none).  o [B, G, H, D], lse fp32 [B, G, H] in base-2 units; a token that sees nothing gets o = 0, lse = -inf.
  * With k, v the call also appends them, as moda_b200_paged_append does, and unless k_copy is NULL writes the rows
  * (the key turned) to k_copy, v_copy [B, 1, H, D] as well: a layer's slot of a depth cache.  With rot, q and k are
- * turned: at position seq_lens[b] with k, v, and otherwise at seq_lens[b] - 1, that of the sequence's last row.
+ * turned: at position seq_lens[b] with k, v, and otherwise at seq_lens[b] - 1, that of the sequence's last row (-1 where
+ * there is none: such a query sees depth rows alone).
  * Rows in pages that are none of the pool's are left out and recorded, as are lengths that are negative or
  * more than the table covers; the token's own row too, which is then not copied either unless cache->copy_all is set: a copy
  * that is the next layer's depth row is read there whether the row has a place here or not.  Nothing that the call writes may be among the rows that it reads.
@@ -330,8 +331,9 @@ const char *moda_b200_kernel_name(int kernel_id);
  * wants to know that its results are valid reads it at its next synchronisation point
  * (0 = every launch since the previous read ran to completion).  The paged-cache calls
  * record here what they left out: (2 << 8 | 1) a page that is none of the pool's, (2 << 8 | 2) a
- * length that is negative or more than the table covers (or than the tokens of an append); where both kinds were recorded the next call
- * returns the second.  SYNCHRONISES the device.  The reference has no counterpart (Triton kernels do not spin on barriers
+ * length that is negative or more than the table covers (or than the tokens of an append, or the positions of
+ * the depth rows); where both kinds were recorded the next call returns the second.  The word is that of the
+ * current device, which the call SYNCHRONISES.  The reference has no counterpart (Triton kernels do not spin on barriers
  * they could miss).
  */
 int moda_b200_device_status(int *status);

@@ -218,12 +218,13 @@ def tensor_pipe_rates(device_ptr: int, device: int, stream: int = 0) -> None:
 
 
 def device_status() -> int:
-    """Sticky status word of the tcgen05 kernels' bounded waits and of the paged-cache calls; synchronises.
+    """Sticky status word of the tcgen05 kernels' bounded waits and of the paged-cache calls, of the current device; synchronises it.
 
     0 = every launch since the previous read ran to completion.  Non-zero = the first wait that
     expired since then ((1 << 8) | barrier id): that launch returned early and left outputs
     unwritten; or what a paged-cache call left out first ((2 << 8) | 1: a page that is none of the
-    pool's, (2 << 8) | 2: a length that is negative or more than the table covers, or than an append has tokens).
+    pool's, (2 << 8) | 2: a length that is negative or more than the table covers, or than an append
+    has tokens, or than there are positions of depth rows).
     Reading resets the word, so callers poll it at their next synchronisation point."""
     v = ctypes.c_int(0)
     check(load().moda_b200_device_status(ctypes.byref(v)), "moda_b200_device_status")

@@ -166,7 +166,9 @@ bool too_many_keys(int64_t B, int64_t most_keys) {
 }
 
 // How a decoding call is divided.  The lengths are known on the device alone; what is known here is how long a sequence may be, by
-// the width of its table (and L depth rows).
+// the width of its table (and L depth rows).  A table wider than its sequences costs the one-launch forms: one step over 4095 rows
+// of 8 heads 12.0 us, 14.6 where the table has 131072 positions, 60 sequences of 60 rows 8.2 and 12.5.  Depth rows of several positions count as
+// those of one here: a choice of fewer CTAs for them than they could use, not of a wrong result.
 struct Division { int ctas, cluster; };
 int divide(const moda_problem* pr, int64_t most_rows, Division* out) {
   const int n_sm = sm_count(pr->device);
@@ -181,7 +183,7 @@ int divide(const moda_problem* pr, int64_t most_rows, Division* out) {
     if (units > most) break;
     log_size = next;
   }
-  // A cluster's CTAs may have up to 32 tiles each, or 52 times the part of the device that they fill if that is more: an even division
+  // A cluster's CTAs may have up to 32 tiles of cached and one position's depth rows each, or 52 times the part of the device that they fill if that is more: an even division
   // fills all of it, but takes a second launch.  Rows as long as the table allows, and half of that on average, D = 128, 8 heads (128 CTAs of 296), 28 tiles:
   // 13.2 and 11.4 us against 13.8 and 12.6, 44 tiles: 17.7 and 14.7 against 15.3 and 14.2; 32 heads (256 CTAs), 44 tiles: 19.3 and 16.5
   // against 24.3 and 15.4; 296 heads, 49 tiles: 22.6 and 17.5 against 26.4 and 20.5

@@ -53,8 +53,9 @@ def paged_moda_decode(q: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Ten
     The token sees the ``seq_lens[b]`` rows of its sequence in the cache, its own ``k, v [B, 1, H, D]`` where given (they are
     also appended, as by ``paged_moda_append``; without them its row is the sequence's last), and the depth rows
     ``cached_k, cached_v``: ``[B, L, H, D]`` of its own position, or ``[B, P, L, H, D]`` of positions of its chunk, of which it sees the
-    first ``depth_positions[b]`` (int32; chunk-visible).  With ``rotary`` ``q`` and ``k`` are turned at the token's position;
-    depth rows are used as they are.  ``record_k, record_v [B, 1, H, D]`` (none of the rows that are read) receive the token's row as
+    first ``depth_positions[b]`` (int32; chunk-visible).  With ``rotary`` ``q`` and ``k`` are turned at the token's position:
+    ``seq_lens[b]`` with ``k``, otherwise that of the sequence's last row (-1 where it has none, and sees depth rows alone); depth rows
+    are used as they are.  ``record_k, record_v [B, 1, H, D]`` (none of the rows that are read) receive the token's row as
     written to the cache; a token whose row has no place there leaves them as they are, unless ``record_all``.  A token that sees
     nothing gets ``o = 0``, ``lse = -inf``."""
     r = _cabi.native().paged_decode(q, cache_k, cache_v, block_table, seq_lens, k, v, cached_k, cached_v, depth_positions, scale,
